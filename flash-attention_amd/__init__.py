@@ -17,7 +17,7 @@ import ctypes
 import enum
 import os
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import Any, Dict, Optional, Tuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 REPO_ROOT = os.path.dirname(_HERE)
@@ -72,6 +72,7 @@ ABI_SYMBOLS = (
     "flash_fwd_f32_workspace_bytes", "flash_fwd_query",
     "flash_fwd_query_entry",
     "flash_kernel_type_name",
+    "flash_fwd_packed", "flash_decode_paged", "flash_decode_paged_workspace_bytes", "flash_cache_append",
     "flash_hip_last_error", "flash_hip_version", "flash_hip_reload_switches",
 )
 
@@ -105,6 +106,13 @@ def lib() -> ctypes.CDLL:
     L.flash_fwd_query.restype = ctypes.c_int
     L.flash_fwd_query_entry.argtypes = [i64, i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_LaunchInfo)]
     L.flash_fwd_query_entry.restype = ctypes.c_int
+    for name, nargs in (("flash_fwd_packed", 2), ("flash_cache_append", 3)):
+        getattr(L, name).argtypes = [vp] * nargs
+        getattr(L, name).restype = ctypes.c_int
+    L.flash_decode_paged.argtypes = [vp, vp, vp, i64, vp]
+    L.flash_decode_paged.restype = ctypes.c_int
+    L.flash_decode_paged_workspace_bytes.argtypes = [vp, vp]
+    L.flash_decode_paged_workspace_bytes.restype = i64
     L.flash_kernel_type_name.argtypes = [ctypes.c_int]
     L.flash_kernel_type_name.restype = ctypes.c_char_p
     L.flash_hip_last_error.argtypes = []
@@ -209,6 +217,79 @@ def load_pyflash() -> None:
     if not os.path.exists(PYFLASH_PATH):
         raise ImportError(f"{PYFLASH_PATH} not found: run __graft_entry__.build()")
     torch.ops.load_library(PYFLASH_PATH)
+
+
+# ---- serving: packed prompts, a paged key-value cache, one new token at a time ----------------------
+# No counterpart in the reference.  The checks and the launch are in C++ (flash/serving.cpp, reached through
+# torch.ops.pyflash.*): a decoding step is a few microseconds of GPU time, which ctypes would double.
+_serving_ops: Dict[str, Any] = {}
+
+
+def _serving(name: str):
+    op = _serving_ops.get(name)
+    if op is None:
+        import torch
+
+        load_pyflash()
+        op = _serving_ops[name] = getattr(torch.ops.pyflash, name).default
+    return op
+
+
+def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = True, softmax_scale=None, out=None,
+                   sync: bool = True):
+    """Attention over packed prompts: sequences of different lengths one behind the other, grouped heads.
+
+    q ``[total_q, Hq, d]``, k and v ``[total_k, Hkv, d]`` on a HIP device, fp16 or bf16, ``Hq`` a multiple of ``Hkv``
+    (query head h reads K/V head ``h // (Hq // Hkv)``), d a multiple of 8 up to 128; any token and head strides that
+    keep rows on 16-byte boundaries, so slices of one fused projection need no copy.  ``cu_seqlens_q`` (int32,
+    ``[sequences + 1]``, on the device) holds the places where sequences begin and end; ``cu_seqlens_k`` the same for
+    the keys (default: the same places).  With ``causal`` query i of a sequence with nq queries and nk keys sees
+    the keys j <= i + nk - nq: the last query sees the last key, which is what a later piece of a prompt needs.  A
+    query that sees no key gets zeros.  Masked keys and values may hold anything, NaN and infinities included; values
+    that are seen are summed in fp32 before they are divided by the weights' sum (bf16 values beyond 1e30 may overflow).
+
+    Returns a new tensor like q, or ``out``; rows behind the last sequence are left as they were.  No backward
+    pass.  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
+    return _serving("forward_packed")(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, softmax_scale=softmax_scale,
+                                      out=out, sync=sync)
+
+
+def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=None, k_scale=None, v_scale=None, out=None,
+                 return_lse: bool = False, workspace=None, sync: bool = True):
+    """Attention of one new token of every sequence over a paged key-value cache.
+
+    q ``[sequences, Hq, d]``, fp16 or bf16; caches ``[pages, Hkv, page_size, d]`` of the same type or
+    float8_e4m3fn, with equal strides (a cache kept as ``[pages, page_size, Hkv, d]`` is passed as
+    ``cache.transpose(1, 2)``), ``page_size`` a power of two.  Position j of sequence b lies in page
+    ``page_table[b, j // page_size]``, slot ``j % page_size``; ``seq_lens[b]`` positions hold tokens, the new one
+    among them (:func:`cache_append` comes first).  Both int32 and on the device.  ``k_scale`` and ``v_scale``
+    (float32 ``[Hkv]``, e4m3 caches only) say what a stored 1 stands for.
+
+    A sequence of length 0 gets zeros; pages outside the cache hold no keys.  With ``return_lse`` the result is
+    ``(out, lse)``, lse float32 ``[sequences, Hq]`` the logarithm of the weights' sum (-inf for length 0), with which
+    results over several parts of a context can be joined.  ``workspace``: a tensor of
+    :func:`decode_workspace_bytes` bytes for callers that manage memory themselves; calls that may overlap need
+    one each.  Lengths and pages are read on the device, so a captured graph follows them."""
+    o, lse = _serving("decode_paged")(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, k_scale=k_scale,
+                                      v_scale=v_scale, out=out, return_lse=return_lse, workspace=workspace, sync=sync)
+    return (o, lse) if return_lse else o
+
+
+def decode_workspace_bytes(q, k_cache, page_table) -> int:
+    """Bytes of scratch that :func:`decode_paged` uses for these shapes (values are not looked at)."""
+    return _serving("decode_workspace_bytes")(q, k_cache, page_table)
+
+
+def cache_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, *, k_scale=None, v_scale=None,
+                 sync: bool = True) -> None:
+    """Writes the keys and values of new tokens into the pages of a cache, in place.
+
+    k and v ``[tokens, Hkv, d]``, fp16 or bf16; rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32, on the
+    device; default: one row for each sequence) are the last tokens of sequence b, whose length ``seq_lens[b]`` counts
+    them already.  A 16-bit cache gets the values as they are, a float8_e4m3fn cache the nearest value to
+    ``x / scale`` (ties to even, at most 448).  Rows of no sequence, positions outside the table and pages outside
+    the cache are not written."""
+    _serving("cache_append")(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens, k_scale=k_scale, v_scale=v_scale, sync=sync)
 
 
 # ---- batch x heads sharding across GPUs (one process per GPU) -------------------------------------
@@ -345,7 +426,7 @@ def forward_shard_gather(Qs, Ks, Vs, total_heads: int, kernel_type=KernelType.mm
 
 __all__ = [
     "KernelType", "LaunchInfo", "ABI_SYMBOLS", "ENTRY_F16", "ENTRY_BF16", "ENTRY_F32", "ENTRY_F32_WS", "lib", "to_string", "launch_info", "forward",
-    "load_pyflash", "shard_heads", "forward_shard", "gather_output", "head_chunks",
+    "load_pyflash", "forward_packed", "decode_paged", "decode_workspace_bytes", "cache_append", "shard_heads", "forward_shard", "gather_output", "head_chunks",
     "forward_shard_gather",
     "LIB_PATH", "PYFLASH_PATH", "RUNNER_PATH", "REPO_ROOT",
 ]

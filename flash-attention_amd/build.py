@@ -1,7 +1,7 @@
 """In-tree build of every native artefact (plain compiler invocations, no cmake needed).
 
   flash-attention_amd/lib/libflash_hip.so   HIP kernels + C ABI            (hipcc --offload-arch=gfx950)
-  build/libflash.a                          flash::forward on libtorch     (g++)
+  build/libflash.a                          flash::forward and the serving operators on libtorch (g++)
   build/pyflash/libpyflash.so               torch.ops.pyflash.*            (g++), path as in the reference
   build/runner                              correctness tests / benchmark  (g++)
   tests/native/selftest                     torch-free parity harness      (hipcc host + oracle)
@@ -46,28 +46,48 @@ def _hipcc():
     return "hipcc"
 
 
+# no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip
+HIP_FLAGS = ["-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# Translation units of the library -> (flags of its own, headers).  The attention forward on [B, H, N, d] tensors has
+# no place for NaN; the serving operators have (masked places may hold them).
+HIP_UNITS = {
+    "flash_hip": (["-fno-honor-nans"], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp",
+                                        "cast_f16.hpp", "host.hpp"]),
+    "flash_serve": ([], ["attn_direct.hpp", "attn_paged.hpp", "attn_packed.hpp", "cache_append.hpp",
+                         "serving_index.hpp", "host.hpp"]),
+}
+
+
+def _hip_inputs(unit):
+    return ([os.path.join(HERE, "csrc", unit + ".hip"), os.path.join(ROOT, "include", "flash_hip.h")] +
+            [os.path.join(HERE, "csrc", h) for h in HIP_UNITS[unit][1]])
+
+
 def build_hip_library(force=False):
     out = os.path.join(HERE, "lib", "libflash_hip.so")
-    srcs = glob.glob(os.path.join(HERE, "csrc", "*")) + [os.path.join(ROOT, "include", "flash_hip.h")]
-    if force or _stale(out, srcs):
-        os.makedirs(os.path.dirname(out), exist_ok=True)
-        _run([_hipcc(), f"--offload-arch={ARCH}"] + HIP_FLAGS + ["-fPIC", "-shared",
-              os.path.join(HERE, "csrc", "flash_hip.hip"), "-o", out])
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    os.makedirs(os.path.join(BUILD, "obj"), exist_ok=True)
+    objs = {u: os.path.join(BUILD, "obj", u + ".o") for u in HIP_UNITS}
+
+    def compile_unit(u):
+        if force or _stale(objs[u], _hip_inputs(u)):
+            _run([_hipcc(), f"--offload-arch={ARCH}"] + HIP_FLAGS + HIP_UNITS[u][0] +
+                 ["-fPIC", "-c", os.path.join(HERE, "csrc", u + ".hip"), "-o", objs[u]])
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=4) as ex:
+        list(ex.map(compile_unit, HIP_UNITS))
+    if force or _stale(out, objs.values()):
+        _run([_hipcc(), f"--offload-arch={ARCH}", "-shared"] + list(objs.values()) + ["-o", out])
     return out
 
 
-# no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip
-HIP_FLAGS = ["-O3", "-std=c++17", "-fno-honor-nans", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
-
-def build_device_asm(force=False):
-    """gfx950 assembly of every kernel in the library (same flags as the library itself)."""
-    out = os.path.join(BUILD, "flash_hip.s")
-    srcs = glob.glob(os.path.join(HERE, "csrc", "*")) + [os.path.join(ROOT, "include", "flash_hip.h")]
-    if force or _stale(out, srcs):
+def build_device_asm(force=False, unit="flash_hip"):
+    """gfx950 assembly of every kernel in a translation unit of the library (same flags as the library itself)."""
+    out = os.path.join(BUILD, unit + ".s")
+    if force or _stale(out, _hip_inputs(unit)):
         os.makedirs(BUILD, exist_ok=True)
-        _run([_hipcc(), f"--offload-arch={ARCH}"] + HIP_FLAGS + ["--cuda-device-only", "-S",
-             os.path.join(HERE, "csrc", "flash_hip.hip"), "-o", out])
+        _run([_hipcc(), f"--offload-arch={ARCH}"] + HIP_FLAGS + HIP_UNITS[unit][0] + ["--cuda-device-only", "-S",
+             os.path.join(HERE, "csrc", unit + ".hip"), "-o", out])
     return out
 
 
@@ -117,6 +137,7 @@ def build_torch_targets(force=False):
     hdrs = glob.glob(os.path.join(HERE, "flash", "*.hpp")) + [os.path.join(ROOT, "include", "flash_hip.h")]
     units = {
         "launch": os.path.join(HERE, "flash", "launch.cpp"),
+        "serving": os.path.join(HERE, "flash", "serving.cpp"),
         "pyflash": os.path.join(HERE, "pyflash", "pyflash.cpp"),
         "main": os.path.join(HERE, "main.cpp"),
     }
@@ -126,14 +147,14 @@ def build_torch_targets(force=False):
         if force or _stale(objs[k], [units[k]] + hdrs):
             _run(["g++", "-c", units[k], "-o", objs[k]] + cflags)
 
-    with concurrent.futures.ThreadPoolExecutor(max_workers=3) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=4) as ex:
         list(ex.map(compile_unit, units))
 
     liba = os.path.join(BUILD, "libflash.a")
-    if force or _stale(liba, [objs["launch"]]):
+    if force or _stale(liba, [objs["launch"], objs["serving"]]):
         if os.path.exists(liba):
             os.remove(liba)
-        _run(["ar", "rcs", liba, objs["launch"]])
+        _run(["ar", "rcs", liba, objs["launch"], objs["serving"]])
     origin_lib = "-Wl,-rpath,$ORIGIN/../flash-attention_amd/lib"
     # libtorch_hip asks for "libamdhip64.so" and finds the copy torch bundles; libflash_hip.so and the
     # runner ask for the soname "libamdhip64.so.7".  Point that name at torch's copy too, so that a

@@ -1,0 +1,148 @@
+// Attention over packed prompts: sequences of different lengths one behind the other, grouped heads, causal or not.
+//
+// Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b] .. cu_k[b + 1] - 1; its query i sees key j when
+// j <= i + (keys - queries), i.e. the last query sees the last key.  A query that sees no key gets zeros.
+//
+// The number of query tiles of a call is known to the device only; the grid holds total_q / rows + sequences of them
+// for every head, which is enough whatever the lengths are, and every wave finds its sequence by a scan of cu_q.
+#pragma once
+
+#include "attn_direct.hpp"
+#include "serving_index.hpp"
+
+namespace flash_hip {
+namespace packed {
+
+struct Params {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* o;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;  // bytes
+  int32_t sequences, total_q, total_k, heads, kv_heads, d;
+  int32_t causal;
+  uint32_t tiles;     // query tiles of the grid, per head
+  float scale_log2;   // softmax scale * log2 e
+};
+
+// Query tile `tile` of `rows` rows: its sequence's place in q and k, and its first row inside the sequence
+struct Tile {
+  int32_t q0, nq, k0, nk, row;
+  bool there;
+};
+__device__ __forceinline__ Tile find_tile(const Params& p, uint32_t tile, int32_t rows, int lane) {
+  Tile t{0, 0, 0, 0, 0, false};
+  uint32_t before = 0;
+  for (int32_t b0 = 0; b0 < p.sequences; b0 += 64) {
+    const int32_t b = b0 + lane;
+    Range own_rows{0, 0};
+    if (b < p.sequences) own_rows = sequence_rows(p.cu_q[b], p.cu_q[b + 1], p.total_q);
+    uint32_t sum = (uint32_t)((own_rows.count + rows - 1) / rows);
+    const uint32_t own = sum;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t y = (uint32_t)__shfl_up((int)sum, s);
+      if (lane >= s) sum += y;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > tile);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      t.q0 = __builtin_amdgcn_readfirstlane(__shfl(own_rows.start, at));
+      t.nq = __builtin_amdgcn_readfirstlane(__shfl(own_rows.count, at));
+      t.row = (int32_t)(tile - before - (uint32_t)__builtin_amdgcn_readfirstlane(__shfl((int)(sum - own), at))) * rows;
+      const Range keys = sequence_rows(p.cu_k[b0 + at], p.cu_k[b0 + at + 1], p.total_k);
+      t.k0 = keys.start;
+      t.nk = keys.count;
+      t.there = true;
+      return t;
+    }
+    before += (uint32_t)__builtin_amdgcn_readfirstlane(__shfl((int)sum, 63));
+  }
+  return t;
+}
+
+// 16 query rows of one head by one wave, K and V straight from memory (attn_direct.hpp).
+template <int D, int EK, bool FULL>
+__device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int32_t row0, int32_t head, int lane) {
+  using namespace direct;
+  using S = Step<D, EK, false, 1, 1>;
+  const int n = lane & 15, g = lane >> 4;
+  const int32_t kvh = head / (p.heads / p.kv_heads);
+  const int32_t row = row0 + n;
+  u32x4 qf[1][S::kKS];
+  const char* src = p.q + (int64_t)(t.q0 + (row < t.nq ? row : 0)) * p.q_token + (int64_t)head * p.q_head;
+#pragma unroll
+  for (int ks = 0; ks < S::kKS; ++ks) {
+    const int col = 8 * (4 * ks + g);
+    const bool there = row < t.nq && (FULL || col < p.d);
+    const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
+    qf[0][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
+  }
+  // keys the lane's query sees, and those the last row of the 16 does
+  const int32_t sees = visible_keys(row, t.nq, t.nk, p.causal);
+  const int32_t end = visible_keys(row0 + 15 < t.nq ? row0 + 15 : t.nq - 1, t.nq, t.nk, p.causal);
+  typename S::State st;
+  S::clear(st);
+  const char* kh = p.k + (int64_t)t.k0 * p.k_token + (int64_t)kvh * p.k_head;
+  const char* vh = p.v + (int64_t)t.k0 * p.v_token + (int64_t)kvh * p.v_head;
+  for (int32_t key0 = 0; key0 < end; key0 += S::kKeys) {
+    typename S::Block blk;
+    blk.valid = end - key0 >= S::kKeys ? 0xffffffffull : (1ull << (end - key0)) - 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int32_t key = key0 + 16 * i + n;
+      const char* a = kh + (int64_t)(key < end ? key : key0) * p.k_token;
+#pragma unroll
+      for (int ks = 0; ks < S::kKS; ++ks) {
+        const int col = 8 * (4 * ks + g);
+        const bool in = FULL || col < p.d;
+        blk.k[i][ks] = *(const u32x4*)(a + (in ? col * 2 : 0));
+        if (!in) blk.k[i][ks] = u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int32_t key = key0 + S::v_key(0, g, j);
+      const bool in = FULL || n * S::kE < p.d;
+      blk.v[0][j] = *(const typename S::VWord*)(vh + (int64_t)(key < end ? key : key0) * p.v_token + (in ? n * S::kE * 2 : 0));
+    }
+    S::template run<true>(st, blk, qf, p.scale_log2, lane, sees - key0);
+  }
+  const float l = quad_sum(st.l[0]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (row >= t.nq) return;
+  char* dst = p.o + (int64_t)(t.q0 + row) * p.o_token + (int64_t)head * p.o_head;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = S::kE * (4 * g + i);
+    if (FULL || col < p.d) {
+      typename S::VWord w;
+      if constexpr (S::kE == 8) {
+        w = u32x4{pack2<EK>(st.o[0][0][i] * inv, st.o[0][1][i] * inv), pack2<EK>(st.o[0][2][i] * inv, st.o[0][3][i] * inv),
+                  pack2<EK>(st.o[0][4][i] * inv, st.o[0][5][i] * inv), pack2<EK>(st.o[0][6][i] * inv, st.o[0][7][i] * inv)};
+      } else {
+        w = u32x2{pack2<EK>(st.o[0][0][i] * inv, st.o[0][1][i] * inv), pack2<EK>(st.o[0][2][i] * inv, st.o[0][3][i] * inv)};
+      }
+      *(typename S::VWord*)(dst + col * 2) = w;
+    }
+  }
+}
+
+constexpr int kDirectRows = 64;  // 4 waves x 16
+
+template <int D, int EK, bool FULL>
+__global__ __launch_bounds__(256) void packed_direct_kernel(const Params p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Tile t = find_tile(p, blockIdx.x, kDirectRows, lane);
+  const int32_t row0 = t.row + wave * 16;
+  if (!t.there || row0 >= t.nq) return;
+  attend_rows<D, EK, FULL>(p, t, row0, (int32_t)blockIdx.y, lane);
+#endif
+}
+
+}  // namespace packed
+}  // namespace flash_hip

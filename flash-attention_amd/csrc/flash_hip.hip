@@ -17,6 +17,7 @@
 #include "attn_fwd_mfma.hpp"
 #include "attn_fwd_mfma16.hpp"
 #include "cast_f16.hpp"
+#include "host.hpp"
 #if defined(FLASH_PHASE_STAMPS)
 #include <cstdio>
 #include <vector>
@@ -37,7 +38,7 @@ int forward_f32_scratch(const void* q, const void* k, const void* v, void* o, in
                         float softmax_scale, int kernel_type, void* workspace, int64_t workspace_bytes,
                         void* hip_stream);
 
-thread_local char g_err[512] = "";
+thread_local char g_err[kErrorBytes] = "";
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -632,6 +633,16 @@ int static_scratch_ptr(void** out) {
 
 }  // namespace
 
+namespace flash_hip {
+int set_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+}  // namespace flash_hip
+
 extern "C" {
 
 int flash_fwd_f16(const void* q, const void* k, const void* v, void* o, int64_t B, int64_t H, int64_t N, int64_t d,
@@ -761,7 +772,7 @@ const char* flash_kernel_type_name(int kernel_type) {
 
 const char* flash_hip_last_error(void) { return g_err; }
 
-int flash_hip_version(void) { return 310; }
+int flash_hip_version(void) { return 400; }
 
 int flash_hip_reload_switches(void) {
   publish_switches();

@@ -1,0 +1,74 @@
+// Index arithmetic of the serving kernels: plain functions of the lengths, offsets and page tables that the kernels
+// find in device memory.  They decide what is read and written whatever those hold, and compile for the host as well,
+// where tests walk them through every kind of content.
+#pragma once
+
+#include <cstdint>
+
+#if defined(__HIP__)
+#define FLASH_INDEX __host__ __device__ __forceinline__
+#else
+#define FLASH_INDEX inline
+#endif
+
+namespace flash_hip {
+
+FLASH_INDEX int32_t within(int32_t x, int32_t low, int32_t high) { return x < low ? low : (x > high ? high : x); }
+
+// ---- packed sequences -------------------------------------------------------------------------------------------
+struct Range {
+  int32_t start, count;
+};
+// rows of the sequence between two neighbouring entries of cu_seqlens, cut to the tensor's `total` rows
+FLASH_INDEX Range sequence_rows(int32_t from, int32_t to, int32_t total) {
+  const int32_t start = within(from, 0, total);
+  return Range{start, within(to, start, total) - start};
+}
+// keys that row `row` of a sequence with nq queries and nk keys sees
+FLASH_INDEX int32_t visible_keys(int32_t row, int32_t nq, int32_t nk, bool causal) {
+  return causal ? within(row + (nk - nq) + 1, 0, nk) : nk;
+}
+// The sequence that row t belongs to: the last one that starts at or before t (empty ones share their start with the
+// one behind them); -1: none starts there.  The result is below `sequences` for any content.
+template <typename Offsets>
+FLASH_INDEX int32_t sequence_of(const Offsets& cu, int32_t sequences, int32_t t) {
+  int32_t lo = 0, hi = sequences;
+  while (lo < hi) {
+    const int32_t mid = lo + (hi - lo) / 2;
+    if (cu(mid) <= t) {
+      lo = mid + 1;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo - 1;
+}
+
+// ---- the paged cache --------------------------------------------------------------------------------------------
+struct Pages {
+  int64_t page_stride, slot_stride;  // bytes
+  int32_t num_pages, max_keys, page_shift;
+};
+// byte offset of position `pos` inside a head of the cache, -1 for a page index outside it
+FLASH_INDEX int64_t position_offset(const Pages& c, int32_t page, int32_t pos) {
+  if ((uint32_t)page >= (uint32_t)c.num_pages) return -1;
+  return (int64_t)page * c.page_stride + (int64_t)(pos & ((1 << c.page_shift) - 1)) * c.slot_stride;
+}
+// Position of a token that stands `behind` rows (itself among them) before the end of its sequence of length `len`;
+// -1: outside the table
+FLASH_INDEX int32_t new_position(const Pages& c, int32_t len, int32_t behind) {
+  const int64_t pos = (int64_t)len - behind;
+  return behind > 0 && pos >= 0 && pos < c.max_keys ? (int32_t)pos : -1;
+}
+FLASH_INDEX int32_t cache_length(const Pages& c, int32_t len) { return within(len, 0, c.max_keys); }
+
+// ---- the line of units that decoding workgroups divide among themselves --------------------------------------
+// units of a sequence of n keys; an empty one has a unit too, which writes its zeros
+FLASH_INDEX uint32_t units_of(int32_t n, int32_t unit) { return n <= unit ? 1u : (uint32_t)((n - 1) / unit + 1); }
+// units of every workgroup but the last ones
+FLASH_INDEX uint32_t units_each(uint32_t total, uint32_t workgroups) { return (total - 1) / workgroups + 1; }
+// Place in the workspace for workgroup w's part of the triple that starts at unit `start` of the line: a workgroup
+// holds at most two parts, of the triple it begins with and of the one it ends with.
+FLASH_INDEX uint32_t part_slot(uint32_t w, uint32_t each, uint32_t start) { return 2u * w + (w * each < start ? 1u : 0u); }
+
+}  // namespace flash_hip

@@ -1,12 +1,13 @@
 // torch.ops.pyflash.* for PyTorch-ROCm: the reference's twelve operator names with the schema
 // "(Tensor Q, Tensor K, Tensor V) -> Tensor" (reference pyflash/pyflash.cpp:10-35), each bound to
-// flash::forward with the KernelType the reference binds it to.  Loaded the same way:
+// flash::forward with the KernelType the reference binds it to, and the serving operators.  Loaded the same way:
 //   torch.ops.load_library("build/pyflash/libpyflash.so")   (reference benchmarks/bench.py:12-14)
 #include <torch/extension.h>
 
 #include <string>
 
 #include "../flash/launch.hpp"
+#include "../flash/serving.hpp"
 
 namespace {
 
@@ -41,4 +42,17 @@ TORCH_LIBRARY(pyflash, m) {
   bind<KT::mma_qreg>(m, "mma_qreg");
   bind<KT::mma_qreg_f32x4load>(m, "mma_qreg_vld");
   bind<KT::mma_qreg_async>(m, "mma_qreg_async");
+
+  // the serving operators (flash/serving.hpp); no counterpart in the reference
+  m.def("forward_packed(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor? cu_seqlens_k=None, *, bool causal=True, "
+        "float? softmax_scale=None, Tensor(a!)? out=None, bool sync=True) -> Tensor",
+        &flash::forward_packed);
+  m.def("decode_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor seq_lens, *, "
+        "float? softmax_scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, bool return_lse=False, "
+        "Tensor(b!)? workspace=None, bool sync=True) -> (Tensor, Tensor)",
+        &flash::decode_paged);
+  m.def("decode_workspace_bytes(Tensor q, Tensor k_cache, Tensor page_table) -> int", &flash::decode_workspace_bytes);
+  m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor seq_lens, "
+        "Tensor? cu_seqlens=None, *, Tensor? k_scale=None, Tensor? v_scale=None, bool sync=True) -> ()",
+        &flash::cache_append);
 }

@@ -224,6 +224,104 @@ int flash_fwd_query(int64_t B, int64_t H, int64_t N, int64_t d, int kernel_type,
 int flash_fwd_query_entry(int64_t B, int64_t H, int64_t N, int64_t d, int kernel_type, int entry,
                           flash_launch_info* out);
 
+/* ---- Serving: packed prompts, a paged key-value cache, one new token at a time ------------------------------
+ * No counterpart in the reference (its one operator takes equal lengths, as many K/V heads as query heads and no
+ * mask).  Conventions as above, except:
+ *   - rows are token-major and strided: element (token, head, x) of a tensor lies at token * token_stride +
+ *     head * head_stride + x, strides in elements; the d elements of a row are adjacent.  Rows of 16-bit tensors
+ *     start on 16-byte boundaries, rows of an e4m3 cache on 8-byte ones.
+ *   - query head h reads K/V head h / (q_heads / kv_heads); q_heads is a multiple of kv_heads.
+ *   - d is a multiple of 8, up to 128.
+ *   - offsets, lengths and page tables are device memory and are read by the kernels, so that a captured graph
+ *     follows them.  Whatever they hold, nothing outside the tensors is read or written: offsets are cut to the
+ *     tensors, lengths to the table's reach, and a page index outside the cache means "no keys here".
+ *   - the tensors of a call do not overlap.
+ */
+
+/* Element types.  Values of e4m3: 4 exponent and 3 mantissa bits, no infinities, largest 448. */
+typedef enum flash_hip_dtype { FLASH_F16 = 0, FLASH_BF16 = 1, FLASH_E4M3 = 2 } flash_hip_dtype;
+
+/*
+ * Attention over packed prompts.  Sequence b = 0 .. sequences - 1 has the queries cu_seqlens_q[b] ..
+ * cu_seqlens_q[b + 1] - 1 of q and the keys cu_seqlens_k[b] .. cu_seqlens_k[b + 1] - 1 of k and v; with `causal` its
+ * query i sees key j when j <= i + (its keys - its queries): the last query sees the last key.  A query that sees
+ * no key gets zeros.  Rows of o that belong to no sequence are left as they were.
+ */
+typedef struct flash_packed_args {
+  const void* q;                 /* [total_q, q_heads, d] */
+  const void* k;                 /* [total_k, kv_heads, d] */
+  const void* v;                 /* [total_k, kv_heads, d] */
+  void* o;                       /* [total_q, q_heads, d] */
+  const int32_t* cu_seqlens_q;   /* [sequences + 1] */
+  const int32_t* cu_seqlens_k;   /* [sequences + 1] */
+  int64_t sequences, total_q, total_k;
+  int64_t q_heads, kv_heads, d;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t o_token_stride, o_head_stride;
+  float softmax_scale;           /* positive and finite */
+  int32_t causal;                /* 0 or 1 */
+  int32_t dtype;                 /* FLASH_F16 or FLASH_BF16 */
+} flash_packed_args;
+int flash_fwd_packed(const flash_packed_args* args, void* hip_stream);
+
+/*
+ * A paged cache: position j of sequence b lies in page page_table[b][j / page_size], slot j % page_size.
+ * k_scale and v_scale (e4m3 only; NULL: 1) hold, for each K/V head, what the stored value 1 stands for.
+ */
+typedef struct flash_paged_cache {
+  void* k;                       /* [num_pages, kv_heads, page_size, d]; v has the same strides */
+  void* v;
+  int64_t num_pages, kv_heads, page_size, d;          /* page_size: a power of two */
+  int64_t page_stride, head_stride, slot_stride;      /* elements */
+  const float* k_scale;          /* [kv_heads] */
+  const float* v_scale;          /* [kv_heads] */
+  const int32_t* page_table;     /* [sequences, table_width], rows table_stride entries apart */
+  int64_t sequences, table_width, table_stride;
+  const int32_t* seq_lens;       /* [sequences]: positions that hold a token */
+  int32_t dtype;                 /* type of the cache */
+} flash_paged_cache;
+
+/*
+ * Attention of one new token of every sequence over the cache: q [sequences, q_heads, d] (16-bit, dtype), whose key
+ * and value are in the cache already.  lse (may be NULL): [sequences, q_heads], contiguous, the natural logarithm of
+ * the sum of the weights exp(softmax_scale q.k).  A sequence of length 0 gets zeros and -inf.
+ * `workspace`: device memory, 16-byte aligned, flash_decode_paged_workspace_bytes(...) bytes; scratch, not to be
+ * touched until the call's work has finished, nor shared by calls that may overlap in time (two captured graphs
+ * among them).
+ */
+typedef struct flash_decode_args {
+  const void* q;
+  void* o;                       /* [sequences, q_heads, d] */
+  float* lse;
+  int64_t q_heads;
+  int64_t q_batch_stride, q_head_stride, o_batch_stride, o_head_stride;   /* elements */
+  float softmax_scale;
+  int32_t dtype;                 /* of q and o; a 16-bit cache has the same */
+} flash_decode_args;
+int flash_decode_paged(const flash_decode_args* args, const flash_paged_cache* cache, void* workspace,
+                       int64_t workspace_bytes, void* hip_stream);
+/* -1 (and an error text) for what flash_decode_paged refuses.  Looks at sizes only; does not touch the GPU. */
+int64_t flash_decode_paged_workspace_bytes(const flash_decode_args* args, const flash_paged_cache* cache);
+
+/*
+ * Writes the keys and values of new tokens, k and v [tokens, kv_heads, d], into the cache.  Rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 belong to sequence b (cu_seqlens NULL: row b, tokens == sequences) and take its last
+ * positions, seq_lens[b] counting them already.  Into an e4m3 cache goes the nearest value to x / scale, ties to
+ * even, the largest for what lies beyond it.  Rows of no sequence, positions outside the table and pages outside the
+ * cache are not written; two rows for one position leave either.
+ */
+typedef struct flash_append_args {
+  const void* k;
+  const void* v;
+  int64_t tokens;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;   /* elements */
+  const int32_t* cu_seqlens;     /* [sequences + 1] or NULL */
+  int32_t dtype;                 /* FLASH_F16 or FLASH_BF16; a 16-bit cache has the same */
+} flash_append_args;
+int flash_cache_append(const flash_append_args* args, const flash_paged_cache* cache, void* hip_stream);
+
 /* Name of a kernel type as the reference's to_string prints it (flash/launch.hpp:28-46); NULL if
  * out of range. */
 const char* flash_kernel_type_name(int kernel_type);
@@ -232,8 +330,8 @@ const char* flash_kernel_type_name(int kernel_type);
  * failing call on the same thread. */
 const char* flash_hip_last_error(void);
 
-/* Library version, major*10000 + minor*100 + patch.  310 (padded route for d % 8 != 0 behind
- * flash_fwd_f32_ws; no interface change); flash_launch_info unchanged since 200 (which
+/* Library version, major*10000 + minor*100 + patch.  400 (packed prompts, decoding over a paged cache; nothing
+ * that was there changed); flash_launch_info unchanged since 200 (which
  * appended `persistent`: callers built against 100 must be recompiled, the query functions write the
  * whole structure). */
 int flash_hip_version(void);

@@ -1,0 +1,224 @@
+"""GPU: attention over packed prompts (fa.forward_packed) against a plain float64 form, head by head.  The bounds are
+derived from the kernels' arithmetic in serving_reference.bound."""
+import math
+
+import pytest
+import torch
+
+import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def make(q_lens, k_lens, hq, hk, d, dtype, seed=0, fused=False):
+    gen = torch.Generator().manual_seed(seed)
+    tq, tk = sum(q_lens), sum(k_lens)
+    if fused:
+        x = torch.randn(tq, hq + 2 * hk, d, generator=gen).to(dtype)
+        return x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:], x
+    q = torch.randn(tq, hq, d, generator=gen).to(dtype)
+    k, v = (torch.randn(tk, hk, d, generator=gen).to(dtype) for _ in range(2))
+    return q, k, v, None
+
+
+def call(fa, q, k, v, q_lens, k_lens=None, **more):
+    cu_k = None if k_lens is None else ref.offsets(k_lens).cuda()
+    return fa.forward_packed(q.cuda(), k.cuda(), v.cuda(), ref.offsets(q_lens).cuda(), cu_k, **more)
+
+
+CASES = [
+    # q_lens, k_lens (None: the same), Hq, Hkv, d, dtype
+    ([1], None, 1, 1, 64, F16),
+    ([2, 1, 3], None, 2, 1, 128, BF16),
+    ([17], None, 4, 2, 64, BF16),
+    ([63, 64, 65, 1, 0, 31, 32, 33], None, 3, 1, 128, F16),
+    ([255, 256, 257], None, 2, 2, 128, BF16),
+    ([255, 256, 257, 511], None, 2, 1, 64, F16),
+    ([700, 13, 1100], None, 4, 2, 128, F16),
+    ([300, 5], None, 6, 2, 40, BF16),
+    ([129, 140], None, 5, 5, 72, F16),
+    ([90], None, 2, 1, 8, BF16),
+    ([200, 333], None, 7, 1, 112, BF16),
+    # keys that reach back before the first query: later pieces of prompts
+    ([5, 64, 300], [700, 129, 301], 4, 2, 128, BF16),
+    ([1, 1, 1, 1], [1, 64, 65, 999], 4, 1, 64, F16),
+    ([77], [1357], 2, 2, 96, F16),
+    # more queries than keys: the first ones see nothing; sequences without keys, without queries
+    ([10, 300, 70, 0, 33], [4, 40, 0, 50, 33], 2, 1, 128, F16),
+    ([130], [1], 2, 2, 64, BF16),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"q{'-'.join(map(str, c[0]))}_k{c[1] and '-'.join(map(str, c[1]))}_{c[2]}x{c[3]}_d{c[4]}_{str(c[5])[6:]}")
+def test_against_float64(fa, case, causal):
+    q_lens, k_lens, hq, hk, d, dtype = case
+    q, k, v, _ = make(q_lens, k_lens or q_lens, hq, hk, d, dtype, seed=sum(q_lens))
+    got = call(fa, q, k, v, q_lens, k_lens, causal=causal)
+    assert got.dtype == dtype and got.shape == q.shape and got.is_contiguous()
+    ref.check_packed(got, q, k, v, q_lens, k_lens or q_lens, causal, d ** -0.5)
+
+
+def test_many_short_sequences(fa):
+    lens = [n % 5 for n in range(200)] + [40]
+    q, k, v, _ = make(lens, lens, 2, 1, 64, BF16, seed=3)
+    ref.check_packed(call(fa, q, k, v, lens), q, k, v, lens, lens, True, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype", [(8, 2, 128, BF16), (4, 4, 64, F16)])
+def test_long_prompt(fa, hq, hk, d, dtype):
+    lens = [4099, 700]
+    q, k, v, _ = make(lens, lens, hq, hk, d, dtype, seed=9)
+    ref.check_packed(call(fa, q, k, v, lens), q, k, v, lens, lens, True, d ** -0.5, heads=[0, hq - 1])
+
+
+def test_slices_of_a_fused_projection_and_strided_output(fa):
+    lens, hq, hk, d = [150, 260], 4, 2, 128
+    q, k, v, whole = make(lens, lens, hq, hk, d, F16, seed=4, fused=True)
+    x = whole.cuda()
+    room = torch.full((sum(lens), hq + 1, d), 7.0, dtype=F16, device="cuda")
+    out = room[:, :hq]
+    got = fa.forward_packed(x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:], ref.offsets(lens).cuda(), out=out)
+    assert got.data_ptr() == room.data_ptr() and bool((room[:, hq] == 7.0).all())
+    ref.check_packed(out, q, k, v, lens, lens, True, d ** -0.5)
+    # head-major tensors, as the other operators of this package take them
+    t = [a.transpose(0, 1).contiguous().cuda().transpose(0, 1) for a in (q, k, v)]
+    assert torch.equal(fa.forward_packed(*t, ref.offsets(lens).cuda()), out)
+
+
+def test_rows_behind_the_last_sequence_are_left_as_they_were(fa):
+    lens, pad = [100, 33], 91
+    q, k, v, _ = make([sum(lens) + pad], [sum(lens) + pad], 2, 1, 128, BF16, seed=5)
+    k[sum(lens):] = float("nan")
+    v[sum(lens):] = float("inf")
+    out = torch.full_like(q, 3.0).cuda()
+    call(fa, q, k, v, lens, out=out)
+    assert bool((out[sum(lens):] == 3.0).all())
+    ref.check_packed(out[:sum(lens)], q[:sum(lens)], k[:sum(lens)], v[:sum(lens)], lens, lens, True, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF16), (64, F16), (72, BF16)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf"), "lowest"])
+def test_masked_places_may_hold_anything(fa, d, dtype, poison):
+    """Keys and values that a query does not see do not reach it, whatever they hold, although they share a tile with
+    some it sees; those that see a non-finite value get what the formula gives."""
+    lens = [333, 290]
+    q, k, v, _ = make(lens, lens, 2, 1, d, dtype, seed=6)
+    bad = torch.finfo(dtype).min if poison == "lowest" else poison
+    for row in (40, 201, 330, 333 + 250):
+        v[row, 0, 3::7] = bad
+    got = call(fa, q, k, v, lens)
+    ref.check_packed(got, q, k, v, lens, lens, True, d ** -0.5)
+    k[332] = bad                  # the last key of the first sequence: only the last query sees it
+    got2 = call(fa, q, k, v, lens)
+    assert torch.equal(got2[:332].view(torch.int16), got[:332].view(torch.int16))
+    assert torch.equal(got2[333:].view(torch.int16), got[333:].view(torch.int16))
+
+
+def test_scores_far_apart(fa):
+    """Rows whose largest score stands far above the first ones seen, and far below."""
+    lens, d = [600], 128
+    q, k, v, _ = make(lens, lens, 2, 2, d, F16, seed=7)
+    k *= 0.2
+    for j, gain in ((70, 4.0), (200, 12.0), (401, 25.0), (599, 40.0)):
+        k[j] = q[j] * (gain / 11.0)
+    ref.check_packed(call(fa, q, k, v, lens), q, k, v, lens, lens, True, d ** -0.5)
+    ref.check_packed(call(fa, q, -k, v, lens), q, -k, v, lens, lens, True, d ** -0.5)
+
+
+def test_scale_argument(fa):
+    lens = [50]
+    q, k, v, _ = make(lens, lens, 1, 1, 64, BF16, seed=8)
+    for scale in (0.03, 0.5):
+        ref.check_packed(call(fa, q, k, v, lens, softmax_scale=scale), q, k, v, lens, lens, True, scale)
+
+
+def test_offsets_beyond_the_tensors_stay_inside(fa):
+    """Offsets are cut to the tensors: a sequence that runs past the end ends there, one that runs backwards is empty."""
+    q, k, v, _ = make([64], [64], 1, 1, 64, F16, seed=10)
+    out = torch.full_like(q, 5.0).cuda()
+    cu = torch.tensor([0, 20, 10, 500], dtype=torch.int32).cuda()
+    fa.forward_packed(q.cuda(), k.cuda(), v.cuda(), cu, out=out)
+    # sequences: rows 0..20, nothing, rows 10..64 (which overwrite the first one's rows 10..20)
+    ref.check_packed(out[:10], q[:10], k[:10], v[:10], [10], [10], True, 0.125)
+    whole = ref.attention(q[10:, 0], k[10:, 0], v[10:, 0], ref.visible_keys(54, 54, True), 0.125)
+    ref.assert_within(out[20:, 0], whole[0][10:], ref.bound(whole[0], whole[2], whole[3], 54, 64, F16, True)[10:], "cut sequence")
+
+
+def test_empty_calls(fa):
+    q = torch.empty(0, 4, 64, dtype=F16, device="cuda")
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert fa.forward_packed(q, q[:, :2], q[:, :2], cu).shape == (0, 4, 64)
+    q = torch.randn(5, 4, 64, device="cuda").half()
+    none = q[:0, :2]
+    out = fa.forward_packed(q, none, none, torch.tensor([0, 5], dtype=torch.int32, device="cuda"),
+                            torch.tensor([0, 0], dtype=torch.int32, device="cuda"))
+    assert bool((out == 0).all())
+
+
+def test_captured_and_replayed_with_other_lengths(fa):
+    """The lengths are read on the device: one graph serves every split of the same rows."""
+    total, hq, hk, d = 640, 4, 2, 128
+    q, k, v, _ = make([total], [total], hq, hk, d, BF16, seed=11)
+    qd, kd, vd, cu = q.cuda(), k.cuda(), v.cuda(), ref.offsets([300, 340]).cuda()
+    out = torch.empty_like(qd)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fa.forward_packed(qd, kd, vd, cu, out=out, sync=False)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            fa.forward_packed(qd, kd, vd, cu, out=out, sync=False)
+    for lens in ([300, 340], [640, 0], [1, 639], [320, 320]):
+        cu.copy_(ref.offsets(lens))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, fa.forward_packed(qd, kd, vd, cu)), lens
+    ref.check_packed(out, q, k, v, [320, 320], [320, 320], True, d ** -0.5, heads=[1])
+
+
+def test_runs_on_the_current_stream(fa):
+    lens = [512]
+    q, k, v, _ = make(lens, lens, 4, 4, 128, F16, seed=12)
+    want = call(fa, q, k, v, lens)
+    side = torch.cuda.Stream()
+    src = [x.cuda() for x in (q, k, v)]
+    cu = ref.offsets(lens).cuda()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        moved = [torch.empty_like(x) for x in src]
+        for a, b in zip(moved, src):
+            a.copy_(b)              # behind this on the same stream, in front of it on any other
+        got = fa.forward_packed(*moved, cu, sync=False)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_same_bits_every_time(fa):
+    lens = [1000, 300]
+    q, k, v, _ = make(lens, lens, 4, 2, 128, BF16, seed=13)
+    first = call(fa, q, k, v, lens)
+    for _ in range(3):
+        assert torch.equal(call(fa, q, k, v, lens), first)
+
+
+def test_one_piece_or_several(fa):
+    """A prompt worked off in pieces, each over all keys so far, gives the rows of the whole."""
+    n, hq, hk, d = 700, 4, 2, 64
+    q, k, v, _ = make([n], [n], hq, hk, d, F16, seed=14)
+    for a, b in ((0, 256), (256, 257), (257, 700)):
+        part = call(fa, q[a:b], k[:b], v[:b], [b - a], [b])
+        ref.check_packed(part, q[a:b], k[:b], v[:b], [b - a], [b], True, d ** -0.5, heads=[0, 3])
+
+
+def test_needs_no_gradient(fa):
+    q = torch.randn(4, 2, 64, device="cuda").half().requires_grad_()
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="no backward"):
+        fa.forward_packed(q, q, q, cu)
+    with torch.no_grad():
+        out = fa.forward_packed(q, q, q, cu)
+    assert not out.requires_grad and math.isfinite(float(out.float().sum()))
