@@ -391,11 +391,21 @@ __device__ __forceinline__ void mask_tile(f32x4& s, int kv_tile0, int N, int lan
   }
 }
 
+// Keys that the lane's query of query block q sees: all N of them, or a number of its own for each query (causal
+// masks; block q holds the queries 64 q behind those of block 0).
+struct QueryLimit {
+  int first;  // of the lane's query in block 0
+};
+__device__ __forceinline__ int key_limit(int N, int) { return N; }
+__device__ __forceinline__ int key_limit(const QueryLimit& l, int q) { return l.first + 64 * q; }
+
 // One pipeline step: QK(j+1) (32 MFMAs), PV(j-1) (32 MFMAs), exp(j), in-lane max(j+1).
 //   s_cur/s_nxt[kb][q]: S^T tiles of key block kb (16 keys) and query block q (16 queries)
 //   p_prev/p_cur[q]:    P^T fragments (32 keys) of query block q
+// Where the first query blocks no longer see the keys (the end of a causal item), QK0, EX0 and PV0 name the first
+// block that takes part in the three stages; MASK_Q >= 0: only this block's scores need the mask.
 template <int D, bool HAS_QK, bool HAS_PRELOAD, bool MASKED, int PV_MODE = kPvAccumulate, int EK = kF16, bool TRACK = true,
-          typename Hook>
+          int QK0 = 0, int EX0 = 0, int PV0 = 0, int MASK_Q = -1, typename Hook, typename Limit>
 __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off, uint32_t vb_off, uint32_t kb_next_off,
                                               const LaneAddr<D>& la, const f32x4 (&bias)[kQ16],
                                               const f16x8 (&qf)[kQ16][Cfg<D>::kKS], f16x8 (&ka)[4],
@@ -403,7 +413,7 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
                                               f32x4 (&s_nxt)[2][kQ16], const f16x8 (&p_prev)[kQ16],
                                               f16x8 (&p_cur)[kQ16], float& mx_all, f32x4 (&lsum)[kQ16],
                                               const ScaleSplit sc, const uint64_t pending, uint64_t& vote,
-                                              int kv_next0, int N, int lane) {
+                                              int kv_next0, const Limit& limit, int lane) {
   constexpr int kKS = Cfg<D>::kKS, kDv16 = Cfg<D>::kDv16;
   constexpr int QK_SLOTS = 2 * kKS * kQ16;  // 32 (D = 128), 16 (D = 64)
   constexpr int PV_SLOTS = kDv16 * kQ16;    // 32, 16
@@ -432,7 +442,7 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
   };
   auto finish = [&](int g) __attribute__((always_inline)) {
     const int q = g / 8, e = g % 8;
-    if ((g & 7) == 1 && g >= 9) group_add(g / 8 - 1);
+    if ((g & 7) == 1 && g / 8 - 1 >= EX0) group_add(g / 8 - 1);
     if ((g & 1) != 0 && !(kKnock & 8)) {
       f16x2 w = __builtin_bit_cast(f16x2, pack2<EK>(t_exp_prev, t_exp));
       pin(w);
@@ -459,8 +469,9 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
   auto exp_share = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = n * ELEMS / SLOTS; g < (n + 1) * ELEMS / SLOTS; ++g) {
-      if (g > 0) finish(g - 1);
-      if (g == 0) x_cur = scaled(0);
+      if (g > 8 * EX0) finish(g - 1);
+      if (g < 8 * EX0) continue;
+      if (g == 8 * EX0) x_cur = scaled(g);
       t_exp = (kKnock & 1) ? x_cur : fast_exp2(x_cur);
       asm volatile("" : "+v"(t_exp));
       if (g + 1 < ELEMS) x_nxt = scaled(g + 1);
@@ -471,15 +482,17 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
   // whether ANY score of the wave exceeds the deferral threshold (the rare path works out which query
   // moved).  Value v = 8q + e is register e % 4 of tile e / 4 of query block q; op 0 folds values 0..2,
   // op u values 2u+1 and 2u+2, the last op value 31.
-  auto score = [&](int v) __attribute__((always_inline)) { return s_nxt[(v % 8) / 4][v / 8][v % 4]; };
+  auto score = [&](int v) __attribute__((always_inline)) {
+    return v < 8 * QK0 ? -INFINITY : s_nxt[(v % 8) / 4][v / 8][v % 4];
+  };
   auto max_op = [&](int u) __attribute__((always_inline)) {
     if constexpr (kKnock & 32) return;
     if constexpr (MASKED) {
       // keys beyond N of a query block, right before the chain first touches the block
       const int q_new = u == 0 ? 0 : ((2 * u + 2) % 8 == 0 ? (2 * u + 2) / 8 : -1);
-      if (q_new >= 0 && q_new < kQ16) {
-        mask_tile(s_nxt[0][q_new], kv_next0, N, lane);
-        mask_tile(s_nxt[1][q_new], kv_next0 + 16, N, lane);
+      if (q_new >= QK0 && q_new < kQ16 && (MASK_Q < 0 || q_new == MASK_Q)) {
+        mask_tile(s_nxt[0][q_new], kv_next0, key_limit(limit, q_new), lane);
+        mask_tile(s_nxt[1][q_new], kv_next0 + 16, key_limit(limit, q_new), lane);
       }
     }
     if (u == 0) {
@@ -503,7 +516,8 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
       const int n = f * kQ16 + q;
       const int kb = f / kKS, ks = f % kKS;
       if constexpr (HAS_QK) {
-        if (ks == 0) {
+        if (q < QK0) {
+        } else if (ks == 0) {
           mfma_s_first<EK>(s_nxt[kb][q], ka[f % 4], qf[q][ks], bias[q]);
         } else {
           mfma_s<false, EK>(s_nxt[kb][q], ka[f % 4], qf[q][ks]);
@@ -534,7 +548,8 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
 #pragma unroll
     for (int q = 0; q < kQ16; ++q) {
       const int pslot = b * kQ16 + q;
-      if constexpr (PV_MODE == kPvFirst) {
+      if (q < PV0) {
+      } else if constexpr (PV_MODE == kPvFirst) {
         mfma_o_first0<EK>(o[q][b], va[b % 4], p_prev[q]);
       } else if constexpr (PV_MODE == kPvAccumulate) {
         mfma_o<false, EK>(o[q][b], va[b % 4], p_prev[q]);
@@ -607,7 +622,9 @@ __device__ __forceinline__ void forget_max(float& mx_all) {
   asm volatile("" : "+v"(mx_all));
 }
 
-template <int NB, bool HAS_NEXT, bool PIN = false>
+// OWN_ROWS: only queries whose own maximum passed the threshold move their reference, so that a query's result does not
+// depend on the other queries of its wave (otherwise all queries of the wave move theirs, up, to where they stand).
+template <int NB, bool HAS_NEXT, bool PIN = false, bool OWN_ROWS = false>
 __device__ __forceinline__ void step_end(f32x4 (&o)[kQ16][NB], State (&st)[kQ16], const float mx_all,
                                          f32x4 (&lsum)[kQ16], f32x4 (&bias)[kQ16], f32x4 (&s_nxt)[2][kQ16],
                                          uint64_t& pending, const uint64_t vote, const ScaleSplit sc, int lane) {
@@ -640,7 +657,8 @@ __device__ __forceinline__ void step_end(f32x4 (&o)[kQ16][NB], State (&st)[kQ16]
         const f32x4 &t0 = s_nxt[0][q], &t1 = s_nxt[1][q];
         const float mq = fmaxf(fmaxf(fmaxf(t0[0], t0[1]), fmaxf(t0[2], t0[3])),
                                fmaxf(fmaxf(t1[0], t1[1]), fmaxf(t1[2], t1[3])));
-        const float rise = fmaxf(quad_lane_max(mq, lane), 0.f);  // references only move up
+        const float top = quad_lane_max(mq, lane);
+        const float rise = OWN_ROWS ? (top > sc.thr ? top : 0.f) : fmaxf(top, 0.f);  // references only move up
         st[q].alpha = fast_exp2(-rise * sc.c);
         st[q].mc += rise;
 #pragma unroll

@@ -27,20 +27,25 @@ struct Params {
   float scale_log2;   // softmax scale * log2 e
 };
 
-// Query tile `tile` of `rows` rows: its sequence's place in q and k, and its first row inside the sequence
+// Query tile `tile` of `rows` rows: its sequence's place in q and k, and its first row.  `extent(queries, keys)`: rows
+// that the tiles of a sequence cover together.
 struct Tile {
   int32_t q0, nq, k0, nk, row;
   bool there;
 };
-__device__ __forceinline__ Tile find_tile(const Params& p, uint32_t tile, int32_t rows, int lane) {
+template <typename Extent>
+__device__ __forceinline__ Tile find_tile(const Params& p, uint32_t tile, int32_t rows, int lane, const Extent& extent) {
   Tile t{0, 0, 0, 0, 0, false};
   uint32_t before = 0;
   for (int32_t b0 = 0; b0 < p.sequences; b0 += 64) {
     const int32_t b = b0 + lane;
-    Range own_rows{0, 0};
-    if (b < p.sequences) own_rows = sequence_rows(p.cu_q[b], p.cu_q[b + 1], p.total_q);
-    uint32_t sum = (uint32_t)((own_rows.count + rows - 1) / rows);
-    const uint32_t own = sum;
+    Range q{0, 0}, k{0, 0};
+    if (b < p.sequences) {
+      q = sequence_rows(p.cu_q[b], p.cu_q[b + 1], p.total_q);
+      k = sequence_rows(p.cu_k[b], p.cu_k[b + 1], p.total_k);
+    }
+    const uint32_t own = (uint32_t)((extent(q.count, k.count) + rows - 1) / rows);
+    uint32_t sum = own;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
       const uint32_t y = (uint32_t)__shfl_up((int)sum, s);
@@ -49,34 +54,37 @@ __device__ __forceinline__ Tile find_tile(const Params& p, uint32_t tile, int32_
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      t.q0 = __builtin_amdgcn_readfirstlane(__shfl(own_rows.start, at));
-      t.nq = __builtin_amdgcn_readfirstlane(__shfl(own_rows.count, at));
-      t.row = (int32_t)(tile - before - (uint32_t)__builtin_amdgcn_readfirstlane(__shfl((int)(sum - own), at))) * rows;
-      const Range keys = sequence_rows(p.cu_k[b0 + at], p.cu_k[b0 + at + 1], p.total_k);
-      t.k0 = keys.start;
-      t.nk = keys.count;
+      auto of = [&](int32_t x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, at); };
+      t.q0 = of(q.start);
+      t.nq = of(q.count);
+      t.k0 = of(k.start);
+      t.nk = of(k.count);
+      t.row = (int32_t)(tile - before - (uint32_t)of((int32_t)(sum - own))) * rows;
       t.there = true;
       return t;
     }
-    before += (uint32_t)__builtin_amdgcn_readfirstlane(__shfl((int)sum, 63));
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
   }
   return t;
 }
 
-// 16 query rows of one head by one wave, K and V straight from memory (attn_direct.hpp).
+// 16 query rows of one head by one wave, K and V straight from memory (attn_direct.hpp).  Rows outside the sequence
+// (row0 may be negative) are left out.
 template <int D, int EK, bool FULL>
 __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int32_t row0, int32_t head, int lane) {
   using namespace direct;
   using S = Step<D, EK, false, 1, 1>;
+  if (row0 >= t.nq || row0 + 15 < 0) return;
   const int n = lane & 15, g = lane >> 4;
   const int32_t kvh = head / (p.heads / p.kv_heads);
   const int32_t row = row0 + n;
   u32x4 qf[1][S::kKS];
-  const char* src = p.q + (int64_t)(t.q0 + (row < t.nq ? row : 0)) * p.q_token + (int64_t)head * p.q_head;
+  const bool mine = (uint32_t)row < (uint32_t)t.nq;
+  const char* src = p.q + (int64_t)(t.q0 + (mine ? row : 0)) * p.q_token + (int64_t)head * p.q_head;
 #pragma unroll
   for (int ks = 0; ks < S::kKS; ++ks) {
     const int col = 8 * (4 * ks + g);
-    const bool there = row < t.nq && (FULL || col < p.d);
+    const bool there = mine && (FULL || col < p.d);
     const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
     qf[0][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
   }
@@ -112,7 +120,7 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
   }
   const float l = quad_sum(st.l[0]);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (row >= t.nq) return;
+  if (!mine) return;
   char* dst = p.o + (int64_t)(t.q0 + row) * p.o_token + (int64_t)head * p.o_head;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -130,6 +138,14 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
   }
 }
 
+}  // namespace packed
+
+// the pipelined kernel (flash_packed.hip): whether it takes a call, and its launch
+__attribute__((visibility("hidden"))) bool packed_mfma_takes(const packed::Params& p);
+__attribute__((visibility("hidden"))) int launch_packed_mfma(packed::Params p, bool bf16, hipStream_t stream);
+
+namespace packed {
+
 constexpr int kDirectRows = 64;  // 4 waves x 16
 
 template <int D, int EK, bool FULL>
@@ -137,7 +153,7 @@ __global__ __launch_bounds__(256) void packed_direct_kernel(const Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const Tile t = find_tile(p, blockIdx.x, kDirectRows, lane);
+  const Tile t = find_tile(p, blockIdx.x, kDirectRows, lane, [](int32_t nq, int32_t) { return nq; });
   const int32_t row0 = t.row + wave * 16;
   if (!t.there || row0 >= t.nq) return;
   attend_rows<D, EK, FULL>(p, t, row0, (int32_t)blockIdx.y, lane);

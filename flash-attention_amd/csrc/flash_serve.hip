@@ -310,6 +310,7 @@ int flash_fwd_packed(const flash_packed_args* a, void* hip_stream) {
   p.causal = a->causal;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
   const hipStream_t stream = (hipStream_t)hip_stream;
+  if (flash_hip::packed_mfma_takes(p)) return flash_hip::launch_packed_mfma(p, a->dtype == FLASH_BF16, stream);
   using namespace flash_hip::direct;
   if (a->d <= 64) return a->dtype == FLASH_F16 ? launch_packed_direct<64, kHalf>(p, stream) : launch_packed_direct<64, kBfloat>(p, stream);
   return a->dtype == FLASH_F16 ? launch_packed_direct<128, kHalf>(p, stream) : launch_packed_direct<128, kBfloat>(p, stream);
