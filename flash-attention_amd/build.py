@@ -54,7 +54,8 @@ HIP_UNITS = {
     "flash_hip": (["-fno-honor-nans"], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp",
                                         "cast_f16.hpp", "host.hpp"]),
     "flash_packed": (["-fno-honor-nans"], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp", "attn_direct.hpp",
-                                           "attn_packed.hpp", "attn_packed_mfma.hpp", "serving_index.hpp", "host.hpp"]),
+                                           "attn_packed.hpp", "attn_packed_mfma.hpp", "attn_packed_mfma_body.hpp",
+                                           "serving_index.hpp", "host.hpp"]),
     "flash_serve": ([], ["attn_direct.hpp", "attn_paged.hpp", "attn_packed.hpp", "cache_append.hpp",
                          "serving_index.hpp", "host.hpp"]),
 }

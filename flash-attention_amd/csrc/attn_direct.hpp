@@ -114,6 +114,18 @@ __device__ __forceinline__ float quad_sum(float x) {
   return __uint_as_float(t[0]) + __uint_as_float(t[1]);
 }
 
+// inclusive sum over the 64 lanes of a wave, by the vector ALU's own lane shifts (within rows of 16 lanes, then the last
+// lane of a row into the next, and lane 31 into the upper half)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, true);
+  return x;
+}
+
 // D: head dim rounded up to 64 or 128; CACHE8: K and V are e4m3; NS: 32-key blocks per step; NQ: 16-query blocks
 template <int D, int EK, bool CACHE8, int NS, int NQ>
 struct Step {

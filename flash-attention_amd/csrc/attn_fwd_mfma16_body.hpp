@@ -62,8 +62,8 @@ constexpr bool kRowsumDot2 = false;
 
 constexpr int kQ16 = kRowsPerWave / 16;  // 16-row query blocks per wave
 constexpr int kRing = 3;                 // tiles per LDS ring
-static_assert((kWaves == 4 && kQ16 == 4) || (kWaves == 8 && kQ16 == 2) || (kWaves == 4 && kQ16 == 8),
-              "one wave per SIMD with 64 query rows, two with 32 each, or one with 128 (d = 64 only)");
+static_assert((kWaves == 4 && kQ16 == 4) || (kWaves == 8 && kQ16 == 2) || (kWaves == 4 && kQ16 == 8) || (kWaves == 4 && kQ16 == 2),
+              "one wave per SIMD with 64 query rows, two with 32 each (of one workgroup or two), or one with 128 (d = 64 only)");
 
 template <int D>
 struct Cfg {

@@ -27,46 +27,63 @@ struct Params {
   float scale_log2;   // softmax scale * log2 e
 };
 
-// Query tile `tile` of `rows` rows: its sequence's place in q and k, and its first row.  `extent(queries, keys)`: rows
-// that the tiles of a sequence cover together.
+// A tile of query rows: its sequence's place in q and k, and its first row there
 struct Tile {
   int32_t q0, nq, k0, nk, row;
   bool there;
 };
+// The tiles of all sequences in a row, `rows` query rows each; `extent(queries, keys)`: rows that those of a sequence
+// cover together.  Every wave works this out for itself, 64 sequences at a time.
 template <typename Extent>
-__device__ __forceinline__ Tile find_tile(const Params& p, uint32_t tile, int32_t rows, int lane, const Extent& extent) {
-  Tile t{0, 0, 0, 0, 0, false};
-  uint32_t before = 0;
-  for (int32_t b0 = 0; b0 < p.sequences; b0 += 64) {
+struct TileLine {
+  const Params& p;
+  int32_t rows;
+  int lane;
+  const Extent& extent;
+
+  struct Chunk {
+    Range q, k;
+    uint32_t own, sum;  // tiles of the lane's sequence, and of all sequences up to it
+  };
+  __device__ __forceinline__ Chunk chunk(int32_t b0) const {
+    Chunk c{{0, 0}, {0, 0}, 0, 0};
     const int32_t b = b0 + lane;
-    Range q{0, 0}, k{0, 0};
     if (b < p.sequences) {
-      q = sequence_rows(p.cu_q[b], p.cu_q[b + 1], p.total_q);
-      k = sequence_rows(p.cu_k[b], p.cu_k[b + 1], p.total_k);
+      c.q = sequence_rows(p.cu_q[b], p.cu_q[b + 1], p.total_q);
+      c.k = sequence_rows(p.cu_k[b], p.cu_k[b + 1], p.total_k);
     }
-    const uint32_t own = (uint32_t)((extent(q.count, k.count) + rows - 1) / rows);
-    uint32_t sum = own;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const uint32_t y = (uint32_t)__shfl_up((int)sum, s);
-      if (lane >= s) sum += y;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > tile);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      auto of = [&](int32_t x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, at); };
-      t.q0 = of(q.start);
-      t.nq = of(q.count);
-      t.k0 = of(k.start);
-      t.nk = of(k.count);
-      t.row = (int32_t)(tile - before - (uint32_t)of((int32_t)(sum - own))) * rows;
-      t.there = true;
-      return t;
-    }
-    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    c.own = (uint32_t)((extent(c.q.count, c.k.count) + rows - 1) / rows);
+    c.sum = direct::wave_scan(c.own);
+    return c;
   }
-  return t;
-}
+  // `c`: the first chunk; cut to the grid's tiles (offsets that run backwards could make more of them)
+  __device__ __forceinline__ uint32_t length(const Chunk& c) const {
+    uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)c.sum, 63);
+    for (int32_t b0 = 64; b0 < p.sequences; b0 += 64) n += (uint32_t)__builtin_amdgcn_readlane((int)chunk(b0).sum, 63);
+    return n < p.tiles ? n : p.tiles;
+  }
+  __device__ __forceinline__ Tile tile(uint32_t at, Chunk c) const {
+    Tile t{0, 0, 0, 0, 0, false};
+    uint32_t before = 0;
+    for (int32_t b0 = 0; b0 < p.sequences; b0 += 64) {
+      if (b0 > 0) c = chunk(b0);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + c.sum > at);
+      if (past != 0) {
+        const int l = __builtin_ctzll(past);
+        auto of = [&](int32_t x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, l); };
+        t.q0 = of(c.q.start);
+        t.nq = of(c.q.count);
+        t.k0 = of(c.k.start);
+        t.nk = of(c.k.count);
+        t.row = (int32_t)(at - before - (uint32_t)of((int32_t)(c.sum - c.own))) * rows;
+        t.there = true;
+        return t;
+      }
+      before += (uint32_t)__builtin_amdgcn_readlane((int)c.sum, 63);
+    }
+    return t;
+  }
+};
 
 // 16 query rows of one head by one wave, K and V straight from memory (attn_direct.hpp).  Rows outside the sequence
 // (row0 may be negative) are left out.
@@ -153,7 +170,9 @@ __global__ __launch_bounds__(256) void packed_direct_kernel(const Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const Tile t = find_tile(p, blockIdx.x, kDirectRows, lane, [](int32_t nq, int32_t) { return nq; });
+  auto extent = [](int32_t nq, int32_t) { return nq; };
+  const TileLine<decltype(extent)> line{p, kDirectRows, lane, extent};
+  const Tile t = line.tile(blockIdx.x, line.chunk(0));
   const int32_t row0 = t.row + wave * 16;
   if (!t.there || row0 >= t.nq) return;
   attend_rows<D, EK, FULL>(p, t, row0, (int32_t)blockIdx.y, lane);

@@ -11,35 +11,36 @@
 // Values of keys that some rows of a tile do not see are multiplied by 0 there; where they are infinite or NaN that is
 // wrong, and such rows come out as NaN.  A wave whose output holds one looks at the values of its diagonal tiles and, if
 // they hold one, computes its rows again on the path that keeps them apart (attend_rows).
+//
+// Two layouts (attn_packed_mfma_body.hpp):
+//   m16   64 query rows per wave, 256 per item, one workgroup per compute unit;
+//   m16h  32 query rows per wave, 128 per item, two workgroups per compute unit (80 KB of LDS each at d = 128: three K
+//         tiles and four half tiles of V), whose starts and ends overlap with each other's matrix work.
 #pragma once
 
 #include "attn_fwd_mfma16.hpp"
 #include "attn_packed.hpp"
 
+#define FLASH_M16_NS m16h
+#define FLASH_M16_ROWS 32
+#define FLASH_M16_WAVES 4
+#include "attn_fwd_mfma16_body.hpp"
+#undef FLASH_M16_NS
+#undef FLASH_M16_ROWS
+#undef FLASH_M16_WAVES
+
 namespace flash_hip {
-namespace m16 {
+namespace packed {
 
-constexpr int kPackedRows = 256;
-
-// Query rows [row0, row0 + 256) of a sequence; row0 may be negative in a sequence's first item (see above).
+// How far in front of a sequence's first row its first item begins (see above).
 __device__ __forceinline__ int32_t packed_shift(int32_t nq, int32_t nk, bool causal) {
   return causal ? (nk - nq) & (kBc - 1) : 0;
 }
 
-// A tile iteration: tile t in ring slot SLOT.  Q0 is the first query block that sees tile t, QK_B the first one that sees
-// tile t + 1, PV_A the first one that saw tile t - 1; MASK_A and MASK_B the block whose scores of tile t (second half) and
-// tile t + 1 (first half) are masked; QK_NEXT: there is a tile t + 1, STAGE_V, STAGE_K: one to fetch behind it.
-constexpr int kNoMask = -1, kMaskAll = -2;
-template <int SLOT_, int Q0_, int QK_B_, int PV_A_, int MASK_A_, int MASK_B_, bool STAGE_V_ = true, bool STAGE_K_ = true, bool QK_NEXT_ = true>
-struct TilePlan {
-  static constexpr int SLOT = SLOT_, Q0 = Q0_, QK_B = QK_B_, PV_A = PV_A_, MASK_A = MASK_A_, MASK_B = MASK_B_;
-  static constexpr bool STAGE_V = STAGE_V_, STAGE_K = STAGE_K_, QK_NEXT = QK_NEXT_;
-};
-
 // any of the packed 16-bit values infinite or NaN
-template <int EK>
+template <bool BF16>
 __device__ __forceinline__ bool holds_not_finite(const u32x4& w) {
-  constexpr uint32_t kExponent = EK == kBF16 ? 0x7f80u : 0x7c00u;
+  constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
   bool any = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -48,332 +49,46 @@ __device__ __forceinline__ bool holds_not_finite(const u32x4& w) {
   return any;
 }
 
-// The workgroup's item: (K/V head, tile, head of the group).  K/V heads are dealt to the 8 XCDs in contiguous ranges, so
-// that the readers of a head's K and V share an L2; the longest items (the last rows) of a K/V head come first.
+// The workgroup's item.  K/V heads are taken in batches that hold at least four query heads.  The 8 XCDs form teams of f,
+// as many teams as divide the number of batches, and a team works its batches off one after the other, each XCD every
+// f-th tile, from the last row to the first (the longest items first): the readers of a head's K and V share an L2 or a
+// few, and every XCD gets its share of long and short items.  For every tile come the batch's query heads: an
+// XCD hands its workgroups to its four shader engines in turn, whether they have room or not, so four items of one
+// length in a row keep them evenly loaded (with the eight tiles of one head in a row instead, causal, 1024 rows, 96
+// heads, a compute unit was busy 70 % of the time: one engine got the longest item and the fifth of every head).
 struct Item {
-  packed::Tile it;
+  Tile it;
   int32_t head, kvh;
   int32_t row0;  // first row inside the sequence, may be negative
   int32_t a0;    // keys seen by all rows of the item, a multiple of 64; negative: some rows see none
 };
-__device__ __forceinline__ Item find_item(const packed::Params& p, bool causal, int lane) {
+__device__ __forceinline__ Item find_item(const Params& p, int32_t rows, bool causal, int lane) {
   Item x;
-  const uint32_t bid = blockIdx.x, xcd = bid & 7u, total = p.tiles * (uint32_t)p.heads;
-  const uint32_t per = total >> 3, rem = total & 7u;
-  const uint32_t item = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (bid >> 3);
-  const uint32_t group = (uint32_t)(p.heads / p.kv_heads);
-  const uint32_t kvh = item / (p.tiles * group), in_head = item - kvh * (p.tiles * group), slot = in_head / group;
-  x.kvh = (int32_t)kvh;
-  x.head = (int32_t)(kvh * group + (in_head - slot * group));
-  x.it = packed::find_tile(p, p.tiles - 1 - slot, kPackedRows, lane, [&](int32_t nq, int32_t nk) __attribute__((always_inline)) {
-    return nq > 0 ? nq + packed_shift(nq, nk, causal) : 0;
-  });
+  auto extent = [&](int32_t nq, int32_t nk) __attribute__((always_inline)) { return nq > 0 ? nq + packed_shift(nq, nk, causal) : 0; };
+  const TileLine<decltype(extent)> line{p, rows, lane, extent};
+  const auto c = line.chunk(0);
+  const ItemPlace at = item_place(blockIdx.x, line.length(c), (uint32_t)p.heads, (uint32_t)p.kv_heads);
+  x.it.there = at.there;
+  if (!at.there) return x;
+  x.head = (int32_t)at.head;
+  x.kvh = (int32_t)(at.head / (uint32_t)(p.heads / p.kv_heads));
+  x.it = line.tile(at.tile, c);
   x.row0 = x.it.row - packed_shift(x.it.nq, x.it.nk, causal);
   x.a0 = causal ? x.row0 + x.it.nk - x.it.nq : 0;
   return x;
 }
 
-template <int D, typename TO, bool CAUSAL>
-__device__ __forceinline__ bool packed_item(const packed::Params& p, const Item& item, char* smem_raw);
-
-template <int D, typename TO, bool CAUSAL>
-__global__ __launch_bounds__(kThreads, 1) void attn_fwd_kernel_packed(const packed::Params p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-  bool again;
-  {
-    const Item item = find_item(p, CAUSAL, (int)(threadIdx.x & 63));
-    if (!item.it.there) return;
-    // rows that see no key: at most the first ones of a sequence with more queries than keys
-    again = item.it.nk == 0 || item.a0 < 0;
-    if (!again) again = packed_item<D, TO, CAUSAL>(p, item, smem_raw);
-  }
-  if (again) {
-    // (rare: the arguments are read again here, rather than kept in registers all the while)
-    const packed::Params* late = (const packed::Params*)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(late));
-    int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
-    asm volatile("" : "+v"(lane));
-    const Item item = find_item(*late, CAUSAL, lane);
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-#pragma unroll 1
-    for (int q = 0; q < kQ16; ++q) {
-      packed::attend_rows<D, kElemKindOf<TO> == kBF16 ? direct::kBfloat : direct::kHalf, false>(*late, item.it, item.row0 + 64 * q + 16 * wave,
-                                                                                                item.head, lane);
-    }
-  }
-#endif
-}
-
-// The item on the pipelined body.  True: this wave's rows hold NaN or infinities and so do the values of its diagonal.
-template <int D, typename TO, bool CAUSAL>
-__device__ __forceinline__ bool packed_item(const packed::Params& p, const Item& item, char* smem_raw) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  using C = Cfg<D>;
-  constexpr int EK = kElemKindOf<TO>;
-  constexpr int kKS = C::kKS, kDv16 = C::kDv16, kTileBytes = C::kTileBytes, kBlkBytes = C::kBlkBytes;
-  constexpr int kPiecesPerWave = C::kPiecesPerWave;
-  lds_char* const smem = (lds_char*)smem_raw;
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n16 = lane & 15;
-  const int g = lane >> 4;
-  const int d = p.d;
-  const packed::Tile& it = item.it;
-  const int32_t head = item.head, kvh = item.kvh, row0 = item.row0, a0 = item.a0;
-  // Tiles in front of the end: the diagonal's four (rows that do not exist make some of them idle), or the last one,
-  // which may be partly there.  Tile t lies in ring slot (t + lead) % 3, so that the end begins in slot 0 and every slot is
-  // a constant of the code.
-  const int full = CAUSAL ? a0 / kBc : (it.nk - 1) / kBc;
-  const int lead = (3 - full % 3) % 3;
-  const ScaleSplit sc{p.scale_log2, kDeferLog2 / p.scale_log2};
-
-  const char* const qb = p.q + ((int64_t)it.q0 + row0) * p.q_token + (int64_t)head * p.q_head;
-  char* const ob = p.o + ((int64_t)it.q0 + row0) * p.o_token + (int64_t)head * p.o_head;
-  const char* const kb = p.k + (int64_t)it.k0 * p.k_token + (int64_t)kvh * p.k_head;
-  const char* const vb = p.v + (int64_t)it.k0 * p.v_token + (int64_t)kvh * p.v_head;
-  const uint32_t q_row = (uint32_t)p.q_token, o_row = (uint32_t)p.o_token;
-  const uint32_t k_row = (uint32_t)p.k_token, v_row = (uint32_t)p.v_token;
-  // (offsets beyond the 256 rows are kOob; the launcher sees to it that kOob lies behind them)
-  const __amdgpu_buffer_rsrc_t q_rs = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, kOob, 0x00020000);
-  const __amdgpu_buffer_rsrc_t o_rs = __builtin_amdgcn_make_buffer_rsrc((void*)ob, 0, kOob, 0x00020000);
-
-  lds_char* const k_ring = smem;
-  lds_char* const v_ring = smem + kRing * kTileBytes;
-
-  // staging: as in attn_fwd_kernel_m16; a descriptor covers the rows of one tile that exist, so that rows behind the
-  // sequence read as zeros and 32 bits suffice at every length
-  uint32_t k_off[kPiecesPerWave], v_off[kPiecesPerWave];
-#pragma unroll
-  for (int i = 0; i < kPiecesPerWave; ++i) {
-    const int ci = (wave * kPiecesPerWave + i) * 64 + lane;
-    const int row = ci / C::kChunks;
-    const int src = (ci % C::kChunks) ^ swz<D>(row);
-    k_off[i] = (src * 8 < d) ? (uint32_t)row * k_row + (uint32_t)src * 16u : kOob;
-    v_off[i] = (src * 8 < d) ? (uint32_t)row * v_row + (uint32_t)src * 16u : kOob;
-  }
-  auto tile_srd = [&](const char* base, uint32_t row_bytes, int t) __attribute__((always_inline)) {
-    const int left = it.nk - t * kBc, rows = left < kBc ? left : kBc;
-    return make_srd(base + (int64_t)t * ((int64_t)kBc * row_bytes), rows > 0 ? (uint32_t)(rows - 1) * row_bytes + (uint32_t)d * 2u : 0u);
-  };
-  auto piece = [&](const srd_t srd, const uint32_t (&off)[kPiecesPerWave], lds_char* ring, int slot, int i) __attribute__((always_inline)) {
-    const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ring + slot * kTileBytes + (wave * kPiecesPerWave + i) * 1024));
-    dma_piece(srd, off[i], lds_base);
-  };
-  auto staged_barrier = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
-
-  // ---- Q fragments ------------------------------------------------------------------------------------------
-  f16x8 qf[kQ16][kKS];
-  const int row_n = row0 + 16 * wave + n16;  // the lane's row in query block 0
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-    const bool there = (uint32_t)(row_n + 64 * q) < (uint32_t)it.nq;
-#pragma unroll
-    for (int ks = 0; ks < kKS; ++ks) {
-      const int col = 8 * (ks + kKS * g);
-      const uint32_t off = (there && col < d) ? (uint32_t)(64 * q + 16 * wave + n16) * q_row + (uint32_t)col * 2u : kOob;
-      qf[q][ks] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(q_rs, off, 0, 0));
-    }
-  }
-  {
-    srd_t k0_srd = tile_srd(kb, k_row, 0), v0_srd = tile_srd(vb, v_row, 0);
-    settle_scalars(k0_srd, v0_srd);
-#pragma unroll
-    for (int i = 0; i < kPiecesPerWave; ++i) piece(k0_srd, k_off, k_ring, lead, i);
-#pragma unroll
-    for (int i = 0; i < kPiecesPerWave; ++i) piece(v0_srd, v_off, v_ring, lead, i);
-    srd_t k1_srd = tile_srd(kb, k_row, 1);
-    settle_scalars(k1_srd);
-#pragma unroll
-    for (int i = 0; i < kPiecesPerWave; ++i) piece(k1_srd, k_off, k_ring, lead == 2 ? 0 : lead + 1, i);
-  }
-  // Step 0 multiplies P(-1) = 0 with the second block of "V tile -1": make that finite.
-  for (int i = tid * 16; i < kBlkBytes; i += kThreads * 16) {
-    *FLASH_LDS_CAST(u32x4, v_ring + (lead == 0 ? 2 : lead - 1) * kTileBytes + kBlkBytes + i) = u32x4{0u, 0u, 0u, 0u};
-  }
-  f32x4 o[kQ16][kDv16];
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-#pragma unroll
-    for (int ks = 0; ks < kKS; ++ks) asm volatile("" : "+a"(qf[q][ks]));
-#pragma unroll
-    for (int b = 0; b < kDv16; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[q][b][i] = 0.f;
-      asm volatile("" : "+a"(o[q][b]));
-    }
-  }
-  const LaneAddr<D> la = make_lane_addr<D>(lane, k_ring, v_ring);
-  const QueryLimit limit_causal{row_n + it.nk - it.nq + 1};
-  const auto limit = [&]() __attribute__((always_inline)) {
-    if constexpr (CAUSAL) return limit_causal; else return (int)it.nk;
-  }();
-
-  staged_barrier();
-
-  // ---- prologue: S(0), its row maximum, the first K fragments of block 1 -------------------------------------
-  f32x4 sA[2][kQ16], sB[2][kQ16];
-  f16x8 pA[kQ16], pB[kQ16];
-  f16x8 ka[4];
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) pB[q][j] = (f16)0.f;
-    asm volatile("" : "+v"(pB[q]));
-  }
-  const uint32_t k_first = (uint32_t)(lead * kTileBytes);
-#pragma unroll
-  for (int f = 0; f < 4; ++f) ka[f] = read_k<D>(k_first, la, f / kKS, f % kKS);
-#pragma unroll
-  for (int f = 0; f < 2 * kKS; ++f) {
-#pragma unroll
-    for (int q = 0; q < kQ16; ++q) {
-      if (f % kKS == 0) {
-        mfma_s_first0<EK>(sA[f / kKS][q], ka[f % 4], qf[q][f % kKS]);
-      } else {
-        mfma_s<true, EK>(sA[f / kKS][q], ka[f % 4], qf[q][f % kKS]);
-      }
-    }
-    if (f + 4 < 2 * kKS) {
-      ka[f % 4] = read_k<D>(k_first, la, (f + 4) / kKS, (f + 4) % kKS);
-    } else {
-      ka[f % 4] = read_k<D>(k_first + (uint32_t)kBlkBytes, la, (f + 4 - 2 * kKS) / kKS, (f + 4) % kKS);
-    }
-  }
-  drain_s(sA);
-  State st[kQ16];
-  float mx_all = 0.f;
-  uint64_t vote = 0;
-  f32x4 bias[kQ16];
-  f32x4 lsum[kQ16];
-  uint64_t pending = 0;
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-    mask_tile(sA[0][q], 0, key_limit(limit, q), lane);
-    mask_tile(sA[1][q], 16, key_limit(limit, q), lane);
-    float mx = fmaxf(fmaxf(sA[0][q][0], sA[0][q][1]), fmaxf(sA[0][q][2], sA[0][q][3]));
-    mx = fmaxf(mx, fmaxf(fmaxf(sA[1][q][0], sA[1][q][1]), fmaxf(sA[1][q][2], sA[1][q][3])));
-    const float mc = quad_lane_max(mx, lane);  // every row sees key 0
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sA[0][q][i] -= mc;
-      sA[1][q][i] -= mc;
-      bias[q][i] = -mc;
-    }
-    st[q].mc = mc;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lsum[q][i] = 0.f;
-    pin_lsum<D>(lsum[q], q);
-    st[q].alpha = 1.f;
-  }
-  bias_ready(bias);
-
-  // ---- tile iterations: two steps each ---------------------------------------------------------------------------
-  auto tile_iter = [&](auto plan, int t) __attribute__((always_inline)) {
-    using F = decltype(plan);
-    constexpr int s0 = F::SLOT, s1 = (s0 + 1) % 3, s2 = (s0 + 2) % 3;
-    srd_t k_srd, v_srd;
-    if constexpr (F::STAGE_K) k_srd = tile_srd(kb, k_row, t + 2);
-    if constexpr (F::STAGE_V) v_srd = tile_srd(vb, v_row, t + 1);
-    if constexpr (F::STAGE_K) settle_scalars(k_srd, v_srd); else if constexpr (F::STAGE_V) settle_scalars(v_srd);
-    auto hook1 = [&](int n) __attribute__((always_inline)) {
-      constexpr int kSpacing = (2 * kKS + kDv16) * kQ16 / (2 * kPiecesPerWave);
-      if (n % kSpacing == 1) {
-        const int i = n / kSpacing;
-        if (i < kPiecesPerWave) {
-          if constexpr (F::STAGE_K) piece(k_srd, k_off, k_ring, s2, i);
-        } else if (i < 2 * kPiecesPerWave) {
-          if constexpr (F::STAGE_V) piece(v_srd, v_off, v_ring, s1, i - kPiecesPerWave);
-        }
-      }
-    };
-    auto hook2 = [&](int) __attribute__((always_inline)) {};
-    constexpr uint32_t k_cur = (uint32_t)(s0 * kTileBytes), k_nxt = (uint32_t)(s1 * kTileBytes);
-    constexpr uint32_t v_cur = (uint32_t)(s0 * kTileBytes), v_prv = (uint32_t)(s2 * kTileBytes);
-    pipeline_step<D, true, F::QK_NEXT, F::MASK_A != kNoMask, kPvAccumulate, EK, true, F::Q0, F::Q0, F::PV_A, (F::MASK_A < 0 ? -1 : F::MASK_A)>(
-        hook1, k_cur + kBlkBytes, v_prv + kBlkBytes, k_nxt, la, bias, qf, ka, o, sA, sB, pB, pA, mx_all, lsum, sc, pending, vote, t * kBc + 32,
-        limit, lane);
-    step_end<kDv16, true, false, true>(o, st, mx_all, lsum, bias, sB, pending, vote, sc, lane);
-    pipeline_step<D, F::QK_NEXT, F::QK_NEXT, F::MASK_B != kNoMask, kPvAccumulate, EK, true, F::QK_B, F::Q0, F::Q0, (F::MASK_B < 0 ? -1 : F::MASK_B)>(
-        hook2, k_nxt, v_cur, k_nxt + kBlkBytes, la, bias, qf, ka, o, sB, sA, pA, pB, mx_all, lsum, sc, pending, vote, (t + 1) * kBc, limit, lane);
-    step_end<kDv16, F::QK_NEXT, false, true>(o, st, mx_all, lsum, bias, sA, pending, vote, sc, lane);
-    if constexpr (F::QK_NEXT) staged_barrier();
-  };
-  constexpr int kEndMask = CAUSAL ? 0 : kMaskAll;  // of the end's first tile (idle in front of the other tiles)
-  constexpr int kLastQ = CAUSAL ? 3 : 0;           // first query block that sees the last tile
-  if (full > 0) {
-    // (the first trip begins in the slot of tile 0)
-    for (int t = -lead;;) {
-      if (t >= 0) tile_iter(TilePlan<0, 0, 0, 0, kNoMask, kNoMask>{}, t);
-      ++t;
-      if (t >= 0) tile_iter(TilePlan<1, 0, 0, 0, kNoMask, kNoMask>{}, t);
-      ++t;
-      tile_iter(TilePlan<2, 0, 0, 0, kNoMask, kEndMask>{}, t);
-      if (++t == full) break;
-    }
-  }
-  if constexpr (CAUSAL) {
-    tile_iter(TilePlan<0, 0, 1, 0, 0, 1>{}, full);
-    tile_iter(TilePlan<1, 1, 2, 0, 1, 2>{}, full + 1);
-    tile_iter(TilePlan<2, 2, 3, 1, 2, 3, true, false>{}, full + 2);
-    tile_iter(TilePlan<0, 3, 3, 2, 3, kNoMask, false, false, false>{}, full + 3);
-  } else {
-    tile_iter(TilePlan<0, 0, 0, 0, kMaskAll, kNoMask, false, false, false>{}, full);
-  }
-  // PV of the last block
-  {
-    drain_o(o);
-#pragma unroll
-    for (int b = 0; b < kDv16; ++b) {
-      const f16x8 vf = read_v<D>((uint32_t)kBlkBytes, la, b);
-#pragma unroll
-      for (int q = kLastQ; q < kQ16; ++q) mfma_o<true, EK>(o[q][b], vf, pB[q]);
-    }
-    drain_o(o);
-    drain_lsum<D>(lsum);
-  }
-
-  // ---- epilogue ----------------------------------------------------------------------------------------------
-  bool odd = false;
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-    const float inv = __builtin_amdgcn_rcpf(quad_lane_sum(lsum[q][0], lane));
-    const bool there = (uint32_t)(row_n + 64 * q) < (uint32_t)it.nq;
-#pragma unroll
-    for (int b = 0; b < kDv16; b += 2) {
-      const f32x4 xs = o[q][b] * inv, ys = o[q][b + 1] * inv;
-      const u32x2 xu = {pack2<EK>(xs[0], xs[1]), pack2<EK>(xs[2], xs[3])};
-      const u32x2 yu = {pack2<EK>(ys[0], ys[1]), pack2<EK>(ys[2], ys[3])};
-      u32x4 out;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        auto r = __builtin_amdgcn_permlane16_swap(xu[w], yu[w], false, false);
-        out[w] = r[0];
-        out[2 + w] = r[1];
-      }
-      const int dv = 16 * (b + (g & 1)) + 8 * (g >> 1);
-      const uint32_t off = (there && dv < d) ? (uint32_t)(64 * q + 16 * wave + n16) * o_row + (uint32_t)dv * 2u : kOob;
-      __builtin_amdgcn_raw_buffer_store_b128(out, o_rs, off, 0, 0);
-      if constexpr (CAUSAL) odd |= there && holds_not_finite<EK>(out);
-    }
-  }
-  if constexpr (CAUSAL) {
-    if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-      bool found = false;
-      for (int32_t x = a0 * C::kChunks + lane; x < (a0 + kPackedRows) * C::kChunks; x += 64) {
-        const int32_t key = x / C::kChunks, c = x % C::kChunks;
-        if (key < it.nk && c * 8 < d) found |= holds_not_finite<EK>(*(const u32x4*)(vb + (int64_t)key * p.v_token + c * 16));
-      }
-      return __builtin_amdgcn_ballot_w64(found) != 0;
-    }
-  }
-#endif  // __HIP_DEVICE_COMPILE__
-  return false;
-}
-
-}  // namespace m16
+}  // namespace packed
 }  // namespace flash_hip
+
+#define FLASH_M16_NS m16
+#define FLASH_PACKED_V_BLOCKS 6
+#include "attn_packed_mfma_body.hpp"
+#undef FLASH_M16_NS
+#undef FLASH_PACKED_V_BLOCKS
+
+#define FLASH_M16_NS m16h
+#define FLASH_PACKED_V_BLOCKS 4
+#include "attn_packed_mfma_body.hpp"
+#undef FLASH_M16_NS
+#undef FLASH_PACKED_V_BLOCKS

@@ -57,15 +57,6 @@ template <int D, bool CACHE8>
 constexpr int kUnit = kWaves * 32 * kSub<D, CACHE8>;
 
 __device__ __forceinline__ int32_t length_of(const Params& p, int32_t b) { return cache_length(p.pages, p.lens[b]); }
-// inclusive sum over the lanes of a wave
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint32_t y = (uint32_t)__shfl_up((int)x, s);
-    if (lane >= s) x += y;
-  }
-  return x;
-}
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 // units of all sequences, and of those before sequence `upto`
@@ -77,7 +68,7 @@ __device__ __forceinline__ Line measure_line(const Params& p, int32_t unit, int3
   for (int32_t b0 = 0; b0 < p.batch; b0 += 64) {
     const int32_t b = b0 + lane;
     const uint32_t u = b < p.batch ? units_of(length_of(p, b), unit) : 0u;
-    const uint32_t sum = wave_scan(u, lane);
+    const uint32_t sum = wave_scan(u);
     if (upto >= b0 && upto < b0 + 64) r.before = r.total + uniform((uint32_t)__shfl((int)(sum - u), upto - b0));
     r.total += uniform((uint32_t)__shfl((int)sum, 63));
   }
@@ -109,7 +100,7 @@ __global__ __launch_bounds__(kThreads, NQ <= 2 ? 2 : 1) void decode_kernel(const
   uint32_t first = 0;  // units of the line before sequence b
   for (int32_t b0 = 0; b0 < p.batch; b0 += 64) {
     const uint32_t u = b0 + lane < p.batch ? units_of(length_of(p, b0 + lane), kUnitKeys) * vheads : 0u;
-    const uint32_t sum = wave_scan(u, lane);
+    const uint32_t sum = wave_scan(u);
     const uint64_t past = __builtin_amdgcn_ballot_w64(first + sum > r_begin);
     if (past != 0) {
       const int at = __builtin_ctzll(past);

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cstdlib>
 
 #include "attn_packed_mfma.hpp"
 #include "host.hpp"
@@ -13,41 +14,67 @@ namespace flash_hip {
 
 namespace {
 
-template <int D, typename TO, bool CAUSAL>
-int launch(packed::Params p, hipStream_t stream) {
-  constexpr uint32_t kLds = (uint32_t)m16::Cfg<D>::kLdsBytes;
+using Kernel = void (*)(const packed::Params);
+
+template <Kernel KERNEL, int LDS>
+int launch(const packed::Params& p, hipStream_t stream) {
+  constexpr uint32_t kLds = (uint32_t)LDS;
   static std::atomic<uint64_t> done{0};  // one bit per device: the kernel's LDS size has been set there
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return set_error(FLASH_HIP_ERR_RUNTIME, "hipGetDevice failed: %s", hipGetErrorString(e));
   const bool cached = dev >= 0 && dev < 64;
   if (!cached || !((done.load(std::memory_order_acquire) >> dev) & 1u)) {
-    e = hipFuncSetAttribute((const void*)m16::attn_fwd_kernel_packed<D, TO, CAUSAL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
+    e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
     if (e != hipSuccess) return set_error(FLASH_HIP_ERR_LDS, "Failed to set dynamic shared memory size %u: %s", kLds, hipGetErrorString(e));
     if (cached) done.fetch_or((uint64_t)1 << dev, std::memory_order_release);
   }
-  hipLaunchKernelGGL((m16::attn_fwd_kernel_packed<D, TO, CAUSAL>), dim3(p.tiles * (uint32_t)p.heads), dim3(m16::kThreads), kLds, stream, p);
+  hipLaunchKernelGGL(KERNEL, dim3((uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads)), dim3(m16::kThreads), kLds, stream, p);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FLASH_HIP_ERR_RUNTIME, "flash_fwd_packed: kernel launch failed: %s", hipGetErrorString(e));
   return FLASH_HIP_OK;
 }
 
+template <typename TO>
+struct HalfOut {
+  using type = TO;
+};
+template <>
+struct HalfOut<m16::bf16_out> {
+  using type = m16h::bf16_out;
+};
+
 template <int D, typename TO>
-int launch(const packed::Params& p, hipStream_t stream) {
-  return p.causal ? launch<D, TO, true>(p, stream) : launch<D, TO, false>(p, stream);
+int launch(packed::Params p, hipStream_t stream) {
+  // Long sequences with work for every compute unit take the 256-row items: each K/V tile is fetched and read from LDS by
+  // half as many waves.  Shorter ones take the 128-row items, two workgroups to a compute unit, of which one computes
+  // while the other starts or ends.  Measured, 128-row / 256-row, us: 32 heads of 128 over 8, 16 x 512 rows 67 / 74,
+  // 8 x 1024 88 / 97, 4 x 2048 139 / 141, 2 x 4096 243 / 239, 8192 457 / 442, 16384 1775 / 1719; 32 heads of 64,
+  // 8 x 1024 56 / 66, 2 x 4096 152 / 154, 8192 288 / 282; 160 items of 128 rows (16 heads of 64) 45 / 67.
+  static const char* force = getenv("PK_HALF");
+  const bool half = force ? force[0] == '1' : (int64_t)p.total_k < (int64_t)4096 * p.sequences || (int64_t)p.total_q / m16::kPackedRows * p.heads < 512;
+  // a sequence has at most two tiles more than whole ones among its rows (its first one may be short, and its last one)
+  const int64_t rows = half ? m16h::kPackedRows : m16::kPackedRows;
+  p.tiles = (uint32_t)(p.total_q / rows + 2 * p.sequences);
+  using TH = typename HalfOut<TO>::type;
+  if (half) {
+    return p.causal ? launch<m16h::attn_fwd_kernel_packed<D, TH, true>, m16h::kPackedLds<D>>(p, stream)
+                    : launch<m16h::attn_fwd_kernel_packed<D, TH, false>, m16h::kPackedLds<D>>(p, stream);
+  }
+  return p.causal ? launch<m16::attn_fwd_kernel_packed<D, TO, true>, m16::kPackedLds<D>>(p, stream)
+                  : launch<m16::attn_fwd_kernel_packed<D, TO, false>, m16::kPackedLds<D>>(p, stream);
 }
 
 }  // namespace
 
 bool packed_mfma_takes(const packed::Params& p) {
   const int64_t most = (int64_t)kOob / m16::kPackedRows;  // a row's bytes: 256 of them stay below kOob
-  const int64_t tiles = (int64_t)p.total_q / m16::kPackedRows + 2 * (int64_t)p.sequences;
-  return p.q_token <= most && p.o_token <= most && p.k_token <= most && p.v_token <= most && tiles * p.heads < ((int64_t)1 << 31);
+  const int64_t tiles = (int64_t)p.total_q / m16h::kPackedRows + 2 * (int64_t)p.sequences;
+  return p.q_token <= most && p.o_token <= most && p.k_token <= most && p.v_token <= most && tiles < ((int64_t)1 << 31) &&
+         packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads) < (1ull << 31);
 }
 
 int launch_packed_mfma(packed::Params p, bool bf16, hipStream_t stream) {
-  // a sequence has at most two tiles more than whole ones among its rows (its first one may be short, and its last one)
-  p.tiles = (uint32_t)(p.total_q / m16::kPackedRows + 2 * p.sequences);
   if (p.d <= 64) return bf16 ? launch<64, m16::bf16_out>(p, stream) : launch<64, f16>(p, stream);
   return bf16 ? launch<128, m16::bf16_out>(p, stream) : launch<128, f16>(p, stream);
 }

@@ -44,6 +44,39 @@ FLASH_INDEX int32_t sequence_of(const Offsets& cu, int32_t sequences, int32_t t)
   return lo - 1;
 }
 
+// Which query tile and head workgroup `id` of a grid of packed_grid(...) works on, of `tiles` tiles that there are; every
+// pair comes once.  (The order is explained with the kernel that uses it.)
+struct ItemPlace {
+  uint32_t tile, head;
+  bool there;
+};
+struct ItemTeams {
+  uint32_t batch, batches, teams, members;  // K/V heads a batch; XCDs of a team
+};
+FLASH_INDEX ItemTeams item_teams(uint32_t heads, uint32_t kv_heads) {
+  const uint32_t group = heads / kv_heads, batch = group >= 4 ? 1 : (group == 1 ? 4 : 2), batches = (kv_heads + batch - 1) / batch;
+  const uint32_t divisor = batches & (0u - batches), teams = divisor < 8 ? divisor : 8;
+  return ItemTeams{batch, batches, teams, 8 / teams};
+}
+FLASH_INDEX uint64_t packed_grid(uint64_t tiles, uint32_t heads, uint32_t kv_heads) {
+  const ItemTeams t = item_teams(heads, kv_heads);
+  return 8ull * (t.batches / t.teams) * ((tiles + t.members - 1) / t.members) * t.batch * (heads / kv_heads);
+}
+FLASH_INDEX ItemPlace item_place(uint32_t id, uint32_t tiles, uint32_t heads, uint32_t kv_heads) {
+  const ItemTeams t = item_teams(heads, kv_heads);
+  const uint32_t group = heads / kv_heads, xcd = id & 7u, place = id >> 3;
+  const uint32_t team = xcd & (t.teams - 1), member = xcd / t.teams;
+  // tiles of this XCD: one of every `members`, back and forth, so that their lengths add up alike
+  const uint32_t rounds = tiles / t.members, rest = tiles - rounds * t.members;
+  const uint32_t mine = rounds + (((rounds & 1) ? t.members - 1 - member : member) < rest ? 1 : 0);
+  const uint32_t each = mine * t.batch * group;
+  if (each == 0 || place >= each * (t.batches / t.teams)) return ItemPlace{0, 0, false};
+  const uint32_t nth = place / each, kv0 = (team + nth * t.teams) * t.batch, left = kv_heads - kv0;
+  const uint32_t here = (left < t.batch ? left : t.batch) * group, in_batch = place - nth * each, round = in_batch / here;
+  const uint32_t slot = round * t.members + ((round & 1) ? t.members - 1 - member : member);
+  return ItemPlace{tiles - 1 - slot, kv0 * group + (in_batch - round * here), round < mine};
+}
+
 // ---- the paged cache --------------------------------------------------------------------------------------------
 struct Pages {
   int64_t page_stride, slot_stride;  // bytes

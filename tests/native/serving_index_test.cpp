@@ -48,6 +48,29 @@ static void packed_rows() {
   }
 }
 
+// every (tile, head) pair is the work of exactly one workgroup of the grid, also when fewer tiles exist than the grid
+// was made for
+static void prompt_items() {
+  for (uint32_t kv = 1; kv <= 40; ++kv) {
+    for (uint32_t group : {1u, 2u, 3u, 4u, 5u, 8u, 17u}) {
+      for (uint32_t bound : {1u, 2u, 7u, 16u, 23u}) {
+        for (uint32_t tiles = 0; tiles <= bound; tiles += bound > 7 ? 5 : 1) {
+          const uint64_t grid = packed_grid(bound, kv * group, kv);
+          EXPECT(grid % 8 == 0 && grid < 1u << 20);
+          std::vector<int> seen((size_t)tiles * kv * group, 0);
+          for (uint32_t id = 0; id < grid; ++id) {
+            const ItemPlace x = item_place(id, tiles, kv * group, kv);
+            if (!x.there) continue;
+            EXPECT(x.tile < tiles && x.head < kv * group);
+            seen[(size_t)x.tile * kv * group + x.head] += 1;
+          }
+          for (int n : seen) EXPECT(n == 1);
+        }
+      }
+    }
+  }
+}
+
 static void token_targets() {
   for (int n = 0; n < 20000; ++n) {
     const int32_t seqs = 1 + (int32_t)(rnd() % 9);
@@ -143,6 +166,7 @@ static void the_line() {
 
 int main() {
   packed_rows();
+  prompt_items();
   token_targets();
   cache_places();
   the_line();
