@@ -133,15 +133,13 @@ struct Step {
   static constexpr int kE = D / 16;              // columns of V per lane
   static constexpr int kKeys = 32 * NS;          // keys per step
   static constexpr int kElem = CACHE8 ? 1 : 2;   // bytes of a K or V element
-  typedef typename Words<2 * kElem>::type KWord;             // 8 elements of K
+  static constexpr int kKLoads = CACHE8 ? kKS / 2 : kKS;     // 16-byte loads of a lane per K tile
   typedef typename Words<kE * kElem / 4>::type VWord;        // kE elements of V
 
-  // K and V of one step, as loaded
-  struct Block {
-    KWord k[2 * NS][kKS];
-    VWord v[NS][8];
-    uint64_t valid;  // bit i: key i of the step exists (wave-uniform)
-  };
+  // K and V of one step, as loaded: [16-key tile], [32-key block][key]
+  typedef u32x4 KBlock[2 * NS][kKLoads];
+  typedef VWord VBlock[NS][8];
+
   struct State {
     f32x4 o[NQ][kE];
     float m[NQ], l[NQ];  // l: this lane's keys only
@@ -157,17 +155,22 @@ struct Step {
     }
   }
 
-  // key of the step that lane group g multiplies as element j of sub-block s
-  static __device__ __forceinline__ int v_key(int s, int g, int j) {
-    return 32 * s + 4 * g + (j < 4 ? j : 12 + j);
+  // first of the 8 head-dim elements that lane group g multiplies in k-step ks; a 16-byte load of an 8-bit row holds
+  // those of two k-steps
+  static __device__ __forceinline__ int column(int ks, int g) {
+    return CACHE8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
   }
+  // element (of a row) where load i of a lane's K begins
+  static __device__ __forceinline__ int load_column(int i, int g) { return CACHE8 ? column(2 * i, g) : column(i, g); }
+  // key of the step that lane group g multiplies as element j of block s
+  static __device__ __forceinline__ int v_key(int s, int g, int j) { return 32 * s + 4 * g + (j < 4 ? j : 12 + j); }
 
-  static __device__ __forceinline__ u32x4 k_operand(const KWord& w) {
+  static __device__ __forceinline__ u32x4 k_operand(const u32x4 (&k)[kKLoads], int ks) {
     if constexpr (CACHE8) {
-      const u32x2 a = from_e4m3<EK>(word(w, 0)), b = from_e4m3<EK>(word(w, 1));
+      const u32x2 a = from_e4m3<EK>(k[ks / 2][2 * (ks & 1)]), b = from_e4m3<EK>(k[ks / 2][2 * (ks & 1) + 1]);
       return u32x4{a[0], a[1], b[0], b[1]};
     } else {
-      return w;
+      return k[ks];
     }
   }
 
@@ -175,7 +178,6 @@ struct Step {
     constexpr uint32_t kExponent = EK == kBfloat ? 0x7f80u : 0x7c00u;
     return (half & kExponent) == kExponent;
   }
-
   static __device__ __forceinline__ void drop_not_finite(uint32_t (&r)[8][kE / 2]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -187,195 +189,215 @@ struct Step {
     }
   }
 
-  // `c`: softmax scale * log2 e (and what a unit of an 8-bit K stands for).
-  // LIMIT: the lane's query sees the first `limit` keys of the step only (fewer than one: none).
-  template <bool LIMIT = false>
-  static __device__ __forceinline__ void run(State& st, const Block& b, const u32x4 (&qf)[NQ][kKS], float c, int lane,
-                                             int limit = kKeys) {
-    static_assert(!LIMIT || NQ == 1, "one limit per lane");
-    const int n16 = lane & 15, g = lane >> 4;
+  // Scores of the step's keys, the running maximum and sum, and the weights for the second product.
+  // `c`: softmax scale * log2 e (and what a unit of an 8-bit K stands for).  `valid`: bit i: key i of the step exists
+  // (wave-uniform).  LIMIT: the lane's query sees the first `limit` keys of the step only (fewer than one: none).
+  struct Weights {
+    u32x4 hi[NQ][NS], lo[NQ][NS];
+    float p[2 * NS][4];  // as computed (LIMIT only)
+  };
+  template <bool LIMIT>
+  static __device__ __forceinline__ void weigh(State& st, Weights& w, const KBlock& k, const u32x4 (&qf)[NQ][kKS], uint64_t valid, float c,
+                                               int lane, int limit = kKeys) {
+    const int g = lane >> 4;
     constexpr uint64_t kAll = NS == 1 ? 0xffffffffull : ~0ull;
-    const bool whole = b.valid == kAll;
-    const bool cut = LIMIT && __builtin_amdgcn_ballot_w64(limit < kKeys) != 0;
-    float pr[LIMIT ? 2 * NS : 1][4];  // probabilities, for the values that take the way around the matrix product
-    u32x4 ph[NQ][NS], pl[NQ][NS];
-    {
-      f32x4 s[NQ][2 * NS];
+    f32x4 s[NQ][2 * NS];
 #pragma unroll
-      for (int t = 0; t < 2 * NS; ++t) {
+    for (int t = 0; t < 2 * NS; ++t) {
 #pragma unroll
-        for (int ks = 0; ks < kKS; ++ks) {
-          const u32x4 a = k_operand(b.k[t][ks]);
+      for (int ks = 0; ks < kKS; ++ks) {
+        const u32x4 a = k_operand(k[t], ks);
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            s[q][t] = mfma<EK>(a, qf[q][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[q][t]);
-          }
-        }
+        for (int q = 0; q < NQ; ++q) s[q][t] = mfma<EK>(a, qf[q][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[q][t]);
       }
+    }
+    const bool cut = LIMIT && __builtin_amdgcn_ballot_w64(limit < kKeys) != 0;
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
+    for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-        for (int t = 0; t < 2 * NS; ++t) s[q][t] *= c;
-        if (!whole) {
-#pragma unroll
-          for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (!((b.valid >> (16 * t + 4 * g + i)) & 1)) s[q][t][i] = kMinusInf;
-            }
-          }
-        }
-        if constexpr (LIMIT) {
-          if (cut) {
-#pragma unroll
-            for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (16 * t + 4 * g + i >= limit) s[q][t][i] = kMinusInf;
-              }
-            }
-          }
-        }
-        float mx = s[q][0][0];
-#pragma unroll
-        for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][t][i]);
-        }
-        const float m_new = fmaxf(st.m[q], quad_max(mx));
-        // nothing visible so far: any finite reference will do (every p is 0)
-        const float ref = m_new == kMinusInf ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(st.m[q] - ref);
-        st.m[q] = m_new;
-        float sum = 0.f;
+      for (int t = 0; t < 2 * NS; ++t) s[q][t] *= c;
+      if (valid != kAll) {
 #pragma unroll
         for (int t = 0; t < 2 * NS; ++t) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[q][t][i] = __builtin_amdgcn_exp2f(s[q][t][i] - ref);
-            sum += s[q][t][i];
-            if constexpr (LIMIT) pr[t][i] = s[q][t][i];
+            if (!((valid >> (16 * t + 4 * g + i)) & 1)) s[q][t][i] = kMinusInf;
           }
         }
-        st.l[q] = st.l[q] * alpha + sum;
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+      }
+      if constexpr (LIMIT) {
+        if (cut) {
 #pragma unroll
-          for (int e = 0; e < kE; ++e) st.o[q][e] *= alpha;
-        }
+          for (int t = 0; t < 2 * NS; ++t) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float x = s[q][2 * n + w / 2][2 * (w & 1)], y = s[q][2 * n + w / 2][2 * (w & 1) + 1];
-            const uint32_t hi = pack2<EK>(x, y);
-            ph[q][n][w] = hi;
-            if constexpr (!LIMIT) {
-              const f32x2 back = unpack2<EK>(hi);
-              pl[q][n][w] = pack2<EK>(x - back[0], y - back[1]);
+            for (int i = 0; i < 4; ++i) {
+              if (16 * t + 4 * g + i >= limit) s[q][t][i] = kMinusInf;
             }
+          }
+        }
+      }
+      float mx = s[q][0][0];
+#pragma unroll
+      for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][t][i]);
+      }
+      const float m_new = fmaxf(st.m[q], quad_max(mx));
+      // nothing visible so far: any finite reference will do (every p is 0)
+      const float ref = m_new == kMinusInf ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(st.m[q] - ref);
+      st.m[q] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[q][t][i] = __builtin_amdgcn_exp2f(s[q][t][i] - ref);
+          sum += s[q][t][i];
+          if constexpr (LIMIT) w.p[t][i] = s[q][t][i];
+        }
+      }
+      st.l[q] = st.l[q] * alpha + sum;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int e = 0; e < kE; ++e) st.o[q][e] *= alpha;
+      }
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = s[q][2 * n + i / 2][2 * (i & 1)], y = s[q][2 * n + i / 2][2 * (i & 1) + 1];
+          w.hi[q][n][i] = pack2<EK>(x, y);
+          if constexpr (!LIMIT) {
+            const f32x2 back = unpack2<EK>(w.hi[q][n][i]);
+            w.lo[q][n][i] = pack2<EK>(x - back[0], y - back[1]);
           }
         }
       }
     }
+  }
+
+  // What lies in the place of a key that does not exist may be NaN or infinite, and its weight 0 would not help
+  static __device__ __forceinline__ void clear_missing(VBlock& v, uint64_t valid, int lane) {
+    constexpr uint64_t kAll = NS == 1 ? 0xffffffffull : ~0ull;
+    if (valid == kAll) return;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      // the lane's 8 keys x kE columns as 16-bit words [key][column pair]
-      uint32_t r[8][kE / 2];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        // a key that does not exist has p = 0, but what lies in its place may be NaN or infinite
-        const bool there = whole || ((b.valid >> v_key(n, g, j)) & 1);
+        if (!((valid >> v_key(n, lane >> 4, j)) & 1)) v[n][j] = VWord{};
+      }
+    }
+  }
+
+  // the lane's 8 keys x kE columns of a block as 16-bit words [key][column pair]
+  static __device__ __forceinline__ void v_words(uint32_t (&r)[8][kE / 2], const VWord (&v)[8]) {
 #pragma unroll
-        for (int w = 0; w < (CACHE8 ? kE / 4 : kE / 2); ++w) {
-          const uint32_t x = there ? word(b.v[n][j], w) : 0u;
-          if constexpr (CACHE8) {
-            const u32x2 y = from_e4m3<EK>(x);
-            r[j][2 * w] = y[0];
-            r[j][2 * w + 1] = y[1];
-          } else {
-            r[j][w] = x;
-          }
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int i = 0; i < (CACHE8 ? kE / 4 : kE / 2); ++i) {
+        if constexpr (CACHE8) {
+          const u32x2 y = from_e4m3<EK>(word(v[j], i));
+          r[j][2 * i] = y[0];
+          r[j][2 * i + 1] = y[1];
+        } else {
+          r[j][i] = word(v[j], i);
         }
       }
-      if constexpr (LIMIT) {
-        // A key that some of the 16 queries see and others do not: 0 * infinity in the product would reach
-        // those that do not.  Such values go around it, to the queries that see them only.  (Only steps with a
-        // limit inside look, and these are few: 3 % of the work at 2048 keys.)
-        if (cut) {
-          uint32_t odd = 0;  // bit j: this lane's part of key j is not finite throughout
+    }
+  }
+  template <bool HIGH, bool LOW>
+  static __device__ __forceinline__ void multiply(State& st, const Weights& w, int n, const uint32_t (&r)[8][kE / 2]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+    for (int e = 0; e < kE; ++e) {
+      u32x4 a;
 #pragma unroll
-            for (int w = 0; w < kE / 2; ++w) {
-              if (not_finite(r[j][w]) || not_finite(r[j][w] >> 16)) odd |= 1u << j;
-            }
-          }
-          if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint64_t lanes = __builtin_amdgcn_ballot_w64((odd >> j) & 1);
-#pragma unroll 1
-              for (int from = 0; from < 4; ++from) {
-                if (((lanes >> (16 * from)) & 0xffffu) == 0) continue;
-                const float p = __shfl(pr[2 * n + j / 4][j % 4], n16 + 16 * from);
-                const bool sees = v_key(n, from, j) < limit;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                  for (int w = 0; w < kE / 2; ++w) {
-                    const uint32_t x = (uint32_t)__shfl((int)r[j][w], 16 * from + 4 * g + i);
-                    const f32x2 v = unpack2<EK>(x);
-                    if (sees && not_finite(x)) st.o[0][2 * w][i] += p * v[0];
-                    if (sees && not_finite(x >> 16)) st.o[0][2 * w + 1][i] += p * v[1];
-                  }
-                }
-              }
-            }
-            drop_not_finite(r);
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        a[i] = __builtin_amdgcn_perm(r[2 * i + 1][e / 2], r[2 * i][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
       }
-      // An infinite v: its product with the low part of p (of either sign, or zero) would make NaN of it.  The low part
-      // multiplies finite values only.
-      bool both = true;
-      if constexpr (!LIMIT) {
-        uint16x2 top = {0, 0};
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        if constexpr (HIGH) st.o[q][e] = mfma<EK>(a, w.hi[q][n], st.o[q][e]);
+        if constexpr (LOW) st.o[q][e] = mfma<EK>(a, w.lo[q][n], st.o[q][e]);
+      }
+    }
+  }
+
+  // o += p v with both parts of p.  An infinite v turns into NaN this way (its product with the low part, of either sign
+  // or zero); CAREFUL multiplies the low part with finite values only.
+  template <bool CAREFUL>
+  static __device__ __forceinline__ void accumulate(State& st, const Weights& w, const VBlock& v) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      uint32_t r[8][kE / 2];
+      v_words(r, v[n]);
+      if constexpr (CAREFUL) {
+        multiply<true, false>(st, w, n, r);
+        drop_not_finite(r);
+        multiply<false, true>(st, w, n, r);
+      } else {
+        multiply<true, true>(st, w, n, r);
+      }
+    }
+  }
+  // whether a sum of this wave is NaN
+  static __device__ __forceinline__ bool holds_nan(const State& st) {
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) any |= st.o[q][e][i] != st.o[q][e][i];
+      }
+    }
+    return __builtin_amdgcn_ballot_w64(any) != 0;
+  }
+
+  // o += p v, p rounded once, for keys that some of the 16 queries see and others do not: 0 * infinity in the product
+  // would reach those that do not.  Such values go around it, to the queries that see them only.
+  static __device__ __forceinline__ void accumulate_limited(State& st, const Weights& w, const VBlock& v, int lane, int limit) {
+    static_assert(NQ == 1, "one limit per lane");
+    const int n16 = lane & 15, g = lane >> 4;
+    const bool cut = __builtin_amdgcn_ballot_w64(limit < kKeys) != 0;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      uint32_t r[8][kE / 2];
+      v_words(r, v[n]);
+      if (cut) {
+        uint32_t odd = 0;  // bit j: this lane's part of key j is not finite throughout
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
 #pragma unroll
-          for (int w = 0; w < kE / 2; ++w) {
-            top = __builtin_elementwise_max(top, __builtin_bit_cast(uint16x2, r[j][w] & 0x7fff7fffu));
+          for (int i = 0; i < kE / 2; ++i) {
+            if (not_finite(r[j][i]) || not_finite(r[j][i] >> 16)) odd |= 1u << j;
           }
         }
-        constexpr uint16_t kInfinity = EK == kBfloat ? 0x7f80 : 0x7c00;
-        both = __builtin_amdgcn_ballot_w64(top[0] >= kInfinity || top[1] >= kInfinity) == 0;
-      }
-      auto multiply = [&](auto high, auto low) __attribute__((always_inline)) {
+        if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          u32x4 a;
+          for (int j = 0; j < 8; ++j) {
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64((odd >> j) & 1);
+#pragma unroll 1
+            for (int from = 0; from < 4; ++from) {
+              if (((lanes >> (16 * from)) & 0xffffu) == 0) continue;
+              const float p = __shfl(w.p[2 * n + j / 4][j % 4], n16 + 16 * from);
+              const bool sees = v_key(n, from, j) < limit;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            a[w] = __builtin_amdgcn_perm(r[2 * w + 1][e / 2], r[2 * w][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
+              for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int c = 0; c < kE / 2; ++c) {
+                  const uint32_t x = (uint32_t)__shfl((int)r[j][c], 16 * from + 4 * g + i);
+                  const f32x2 y = unpack2<EK>(x);
+                  if (sees && not_finite(x)) st.o[0][2 * c][i] += p * y[0];
+                  if (sees && not_finite(x >> 16)) st.o[0][2 * c + 1][i] += p * y[1];
+                }
+              }
+            }
           }
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            if constexpr (decltype(high)::value) st.o[q][e] = mfma<EK>(a, ph[q][n], st.o[q][e]);
-            if constexpr (decltype(low)::value) st.o[q][e] = mfma<EK>(a, pl[q][n], st.o[q][e]);
-          }
+          drop_not_finite(r);
         }
-      };
-      constexpr std::true_type yes{};
-      constexpr std::false_type no{};
-      if constexpr (LIMIT) {
-        multiply(yes, no);
-      } else if (both) {
-        multiply(yes, yes);
-      } else {
-        multiply(yes, no);
-        drop_not_finite(r);
-        multiply(no, yes);
       }
+      multiply<true, false>(st, w, n, r);
     }
   }
 };

@@ -100,7 +100,7 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
   const char* src = p.q + (int64_t)(t.q0 + (mine ? row : 0)) * p.q_token + (int64_t)head * p.q_head;
 #pragma unroll
   for (int ks = 0; ks < S::kKS; ++ks) {
-    const int col = 8 * (4 * ks + g);
+    const int col = S::column(ks, g);
     const bool there = mine && (FULL || col < p.d);
     const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
     qf[0][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
@@ -113,27 +113,31 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
   const char* kh = p.k + (int64_t)t.k0 * p.k_token + (int64_t)kvh * p.k_head;
   const char* vh = p.v + (int64_t)t.k0 * p.v_token + (int64_t)kvh * p.v_head;
   for (int32_t key0 = 0; key0 < end; key0 += S::kKeys) {
-    typename S::Block blk;
-    blk.valid = end - key0 >= S::kKeys ? 0xffffffffull : (1ull << (end - key0)) - 1;
+    typename S::KBlock k;
+    typename S::VBlock v;
+    const uint64_t valid = end - key0 >= S::kKeys ? 0xffffffffull : (1ull << (end - key0)) - 1;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int32_t key = key0 + 16 * i + n;
       const char* a = kh + (int64_t)(key < end ? key : key0) * p.k_token;
 #pragma unroll
-      for (int ks = 0; ks < S::kKS; ++ks) {
-        const int col = 8 * (4 * ks + g);
+      for (int x = 0; x < S::kKLoads; ++x) {
+        const int col = S::load_column(x, g);
         const bool in = FULL || col < p.d;
-        blk.k[i][ks] = *(const u32x4*)(a + (in ? col * 2 : 0));
-        if (!in) blk.k[i][ks] = u32x4{0u, 0u, 0u, 0u};
+        k[i][x] = *(const u32x4*)(a + (in ? col * 2 : 0));
+        if (!in) k[i][x] = u32x4{0u, 0u, 0u, 0u};
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int32_t key = key0 + S::v_key(0, g, j);
       const bool in = FULL || n * S::kE < p.d;
-      blk.v[0][j] = *(const typename S::VWord*)(vh + (int64_t)(key < end ? key : key0) * p.v_token + (in ? n * S::kE * 2 : 0));
+      v[0][j] = *(const typename S::VWord*)(vh + (int64_t)(key < end ? key : key0) * p.v_token + (in ? n * S::kE * 2 : 0));
     }
-    S::template run<true>(st, blk, qf, p.scale_log2, lane, sees - key0);
+    S::clear_missing(v, valid, lane);
+    typename S::Weights w;
+    S::template weigh<true>(st, w, k, qf, valid, p.scale_log2, lane, sees - key0);
+    S::accumulate_limited(st, w, v, lane, sees - key0);
   }
   const float l = quad_sum(st.l[0]);
   const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -19,6 +19,9 @@
 #include "attn_direct.hpp"
 #include "serving_index.hpp"
 
+#ifndef FLASH_DW
+#define FLASH_DW 2
+#endif
 namespace flash_hip {
 namespace paged {
 
@@ -75,8 +78,8 @@ __device__ __forceinline__ Line measure_line(const Params& p, int32_t unit, int3
   return r;
 }
 
-template <int D, int EK, bool CACHE8, int NQ, bool FULL>
-__global__ __launch_bounds__(kThreads, NQ <= 2 ? 2 : 1) void decode_kernel(const Params p) {
+template <int D, int EK, bool CACHE8, int NQ, bool FULL, bool PAGE16>
+__global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NS = kSub<D, CACHE8>;
   constexpr int kUnitKeys = kUnit<D, CACHE8>;
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(kThreads, NQ <= 2 ? 2 : 1) void decode_kernel(const
       const char* src = p.q + (int64_t)b * p.q_batch + (int64_t)(kvh * p.group + row0 + (row < rows ? row : 0)) * p.q_head;
 #pragma unroll
       for (int ks = 0; ks < S::kKS; ++ks) {
-        const int col = 8 * (4 * ks + g);
+        const int col = S::column(ks, g);
         const bool there = row < rows && (FULL || col < p.d);
         const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
         qf[q][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
@@ -139,59 +142,103 @@ __global__ __launch_bounds__(kThreads, NQ <= 2 ? 2 : 1) void decode_kernel(const
     const float sc = p.scale_log2 * (CACHE8 && p.k_scale ? p.k_scale[kvh] : 1.f);
     const char* kh = p.k + (int64_t)kvh * p.head_stride;
     const char* vv = p.v + (int64_t)kvh * p.head_stride;
+    const uint32_t slot_stride = (uint32_t)p.pages.slot_stride;
     const int32_t* row_of_table = p.table + (int64_t)b * p.table_stride;
 
-    // page of the lane's key in this wave's step of unit u; -1: no such key
+    // Place in the cache of the lane's key in this wave's step of unit u: its page's entry, then bytes (-1: no such key,
+    // or an entry outside the cache).
     auto page_of = [&](uint32_t u) __attribute__((always_inline)) -> int32_t {
       const int32_t key = (int32_t)u * kUnitKeys + wave * S::kKeys + lane;
       return (lane < S::kKeys && key < len && u < u1) ? row_of_table[key >> p.pages.page_shift] : -1;
     };
-    auto load = [&](typename S::Block& blk, uint32_t u, int32_t page) __attribute__((always_inline)) {
-      const int32_t key = (int32_t)u * kUnitKeys + wave * S::kKeys + lane;
-      // (an entry outside the cache holds no keys; such lanes read slot 0 of page 0 and are masked)
-      const int64_t place = position_offset(p.pages, page, key);
-      blk.valid = __builtin_amdgcn_ballot_w64(place >= 0);
-      const int64_t at = place < 0 ? 0 : place;
+    // (wave-uniform) which keys of the step exist; `at`: where they lie, the start of the cache for the others, which are
+    // read from there and masked
+    auto place = [&](uint32_t u, int32_t page, int64_t& at) __attribute__((always_inline)) -> uint64_t {
+      const int64_t x = position_offset(p.pages, page, (int32_t)u * kUnitKeys + wave * S::kKeys + lane);
+      at = x < 0 ? 0 : x;
+      return __builtin_amdgcn_ballot_w64(x >= 0);
+    };
+    // Row of a key: with pages of at least 16 positions every 16-key tile lies in one page, whose start is a scalar
+    auto tile_start = [&](int64_t at, int t) __attribute__((always_inline)) -> int64_t {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, 16 * t);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), 16 * t);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    };
+    auto load_k = [&](typename S::KBlock& k, int64_t at) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2 * NS; ++t) {
-        const char* src = kh + __shfl(at, 16 * t + n);
+        const char* src = PAGE16 ? kh + tile_start(at, t) : kh + __shfl(at, 16 * t + n);
+        const uint32_t row = PAGE16 ? (uint32_t)n * slot_stride : 0u;
 #pragma unroll
-        for (int ks = 0; ks < S::kKS; ++ks) {
-          const int col = 8 * (4 * ks + g);
+        for (int i = 0; i < S::kKLoads; ++i) {
+          const int col = S::load_column(i, g);
           const bool in = FULL || col < p.d;
-          blk.k[t][ks] = *(const typename S::KWord*)(src + (in ? col * S::kElem : 0));
+          k[t][i] = *(const u32x4*)(src + (row + (uint32_t)((in ? col : 0) * S::kElem)));
           if constexpr (!FULL) {
-            if (!in) blk.k[t][ks] = typename S::KWord{};
+            // (an 8-bit load holds 16 columns, of which the last 8 may lie behind the row)
+            if (!in) k[t][i] = u32x4{0u, 0u, 0u, 0u};
+            if constexpr (CACHE8) {
+              if (in && col + 8 >= p.d) k[t][i][2] = k[t][i][3] = 0u;
+            }
           }
         }
       }
+    };
+    auto load_v = [&](typename S::VBlock& v, int64_t at) __attribute__((always_inline)) {
+      const bool in = FULL || n * S::kE < p.d;
+      const uint32_t col = (uint32_t)(in ? n * S::kE * S::kElem : 0);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool in = FULL || n * S::kE < p.d;
-          blk.v[s][j] = *(const typename S::VWord*)(vv + __shfl(at, S::v_key(s, g, j)) + (in ? n * S::kE * S::kElem : 0));
+          if constexpr (PAGE16) {
+            const uint32_t row = (uint32_t)(4 * g + j % 4) * slot_stride;
+            v[s][j] = *(const typename S::VWord*)(vv + tile_start(at, 2 * s + j / 4) + (row + col));
+          } else {
+            v[s][j] = *(const typename S::VWord*)(vv + __shfl(at, S::v_key(s, g, j)) + col);
+          }
         }
       }
     };
 
+    // K is fetched a step ahead, V at the step's beginning: 16 KB in flight per wave at any time at d = 128
     typename S::State st;
-    S::clear(st);
-    {
-      typename S::Block cur, nxt;
-      int32_t page = page_of(u0);
-      load(cur, u0, page);
-      page = page_of(u0 + 1);
+    auto attend = [&](auto careful) __attribute__((always_inline)) {
+      S::clear(st);
+      typename S::KBlock k, k_next;
+      int64_t at, at_next;
+      uint64_t valid = place(u0, page_of(u0), at), valid_next;
+      int32_t page = page_of(u0 + 1);
+      load_k(k, at);
       for (uint32_t u = u0; u < u1; ++u) {
+        typename S::VBlock v;
+        load_v(v, at);
         const bool more = u + 1 < u1;
         if (more) {
-          load(nxt, u + 1, page);
+          valid_next = place(u + 1, page, at_next);
+          load_k(k_next, at_next);
           page = page_of(u + 2);
         }
-        if (cur.valid != 0) S::run(st, cur, qf, sc, lane);
-        if (more) cur = nxt;
+        if (valid != 0) {
+          typename S::Weights w;
+          S::template weigh<false>(st, w, k, qf, valid, sc, lane);
+          S::clear_missing(v, valid, lane);
+          S::template accumulate<decltype(careful)::value>(st, w, v);
+        }
+        if (more) {
+#pragma unroll
+          for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+            for (int i = 0; i < S::kKLoads; ++i) k[t][i] = k_next[t][i];
+          }
+          at = at_next;
+          valid = valid_next;
+        }
       }
-    }
+    };
+    attend(std::false_type{});
+    // NaN may come from an infinite value (rare: the part is worked out again with care)
+    if (S::holds_nan(st)) attend(std::true_type{});
 
     // ---- the four waves' parts, 16 queries at a time -----------------------------------------------------
     const bool complete = u0 == 0 && u1 == units;

@@ -138,11 +138,10 @@ int plan_decode(const flash_decode_args* a, const flash_paged_cache* c, bool mem
 template <int D, int EK, bool CACHE8, int NQ>
 int launch_decode(const DecodeParams& p, bool join, hipStream_t stream) {
   namespace pg = flash_hip::paged;
-  if (p.d == D) {
-    hipLaunchKernelGGL((pg::decode_kernel<D, EK, CACHE8, NQ, true>), dim3(p.workgroups), dim3(pg::kThreads), 0, stream, p);
-  } else {
-    hipLaunchKernelGGL((pg::decode_kernel<D, EK, CACHE8, NQ, false>), dim3(p.workgroups), dim3(pg::kThreads), 0, stream, p);
-  }
+  const bool page16 = p.pages.page_shift >= 4 && 16 * p.pages.slot_stride < ((int64_t)1 << 31);
+  auto kernel = p.d == D ? (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, true, true> : pg::decode_kernel<D, EK, CACHE8, NQ, true, false>)
+                         : (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, false, true> : pg::decode_kernel<D, EK, CACHE8, NQ, false, false>);
+  hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(pg::kThreads), 0, stream, p);
   CHECK(launched("flash_decode_paged"));
   if (!join) return FLASH_HIP_OK;
   hipLaunchKernelGGL((pg::join_parts_kernel<D, EK, CACHE8, NQ>), dim3((uint32_t)(p.batch * p.kv_heads * p.group)), dim3(pg::kThreads), 0, stream, p);
