@@ -267,9 +267,10 @@ def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=Non
 
     A sequence of length 0 gets zeros; pages outside the cache hold no keys.  With ``return_lse`` the result is
     ``(out, lse)``, lse float32 ``[sequences, Hq]`` the logarithm of the weights' sum (-inf for length 0), with which
-    results over several parts of a context can be joined.  ``workspace``: a tensor of
-    :func:`decode_workspace_bytes` bytes for callers that manage memory themselves; calls that may overlap need
-    one each.  Lengths and pages are read on the device, so a captured graph follows them."""
+    results over several parts of a context can be joined.  ``workspace``: scratch from :func:`decode_workspace`, for
+    callers that manage memory themselves; it serves any number of calls one after the other, calls that may overlap
+    need one each.  (Without it, calls on a stream share one that is kept for the stream, and a captured graph gets its
+    own.)  Lengths and pages are read on the device, so a captured graph follows them."""
     o, lse = _serving("decode_paged")(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, k_scale=k_scale,
                                       v_scale=v_scale, out=out, return_lse=return_lse, workspace=workspace, sync=sync)
     return (o, lse) if return_lse else o
@@ -278,6 +279,13 @@ def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=Non
 def decode_workspace_bytes(q, k_cache, page_table) -> int:
     """Bytes of scratch that :func:`decode_paged` uses for these shapes (values are not looked at)."""
     return _serving("decode_workspace_bytes")(q, k_cache, page_table)
+
+
+def decode_workspace(q, k_cache, page_table):
+    """Zero-filled scratch for :func:`decode_paged` at these shapes (and smaller ones)."""
+    import torch
+
+    return torch.zeros(decode_workspace_bytes(q, k_cache, page_table), dtype=torch.uint8, device=q.device)
 
 
 def cache_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, *, k_scale=None, v_scale=None,
@@ -426,7 +434,7 @@ def forward_shard_gather(Qs, Ks, Vs, total_heads: int, kernel_type=KernelType.mm
 
 __all__ = [
     "KernelType", "LaunchInfo", "ABI_SYMBOLS", "ENTRY_F16", "ENTRY_BF16", "ENTRY_F32", "ENTRY_F32_WS", "lib", "to_string", "launch_info", "forward",
-    "load_pyflash", "forward_packed", "decode_paged", "decode_workspace_bytes", "cache_append", "shard_heads", "forward_shard", "gather_output", "head_chunks",
+    "load_pyflash", "forward_packed", "decode_paged", "decode_workspace", "decode_workspace_bytes", "cache_append", "shard_heads", "forward_shard", "gather_output", "head_chunks",
     "forward_shard_gather",
     "LIB_PATH", "PYFLASH_PATH", "RUNNER_PATH", "REPO_ROOT",
 ]

@@ -189,6 +189,14 @@ struct Step {
     }
   }
 
+  // Bits of block n's keys, shifted so that bits 0..3 and 16..19 are the lane group's (the asm keeps the masked path, which
+  // few steps take, from being worked into the others)
+  static __device__ __forceinline__ uint32_t lane_bits(uint64_t valid, int n, int g) {
+    uint32_t mine = (uint32_t)(valid >> (32 * n)) >> (4 * g);
+    asm volatile("" : "+v"(mine));
+    return mine;
+  }
+
   // Scores of the step's keys, the running maximum and sum, and the weights for the second product.
   // `c`: softmax scale * log2 e (and what a unit of an 8-bit K stands for).  `valid`: bit i: key i of the step exists
   // (wave-uniform).  LIMIT: the lane's query sees the first `limit` keys of the step only (fewer than one: none).
@@ -218,10 +226,14 @@ struct Step {
       for (int t = 0; t < 2 * NS; ++t) s[q][t] *= c;
       if (valid != kAll) {
 #pragma unroll
-        for (int t = 0; t < 2 * NS; ++t) {
+        for (int n = 0; n < NS; ++n) {
+          const uint32_t mine = lane_bits(valid, n, g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!((valid >> (16 * t + 4 * g + i)) & 1)) s[q][t][i] = kMinusInf;
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (!((mine >> (16 * t + i)) & 1)) s[q][2 * n + t][i] = kMinusInf;
+            }
           }
         }
       }
@@ -283,9 +295,10 @@ struct Step {
     if (valid == kAll) return;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
+      const uint32_t mine = lane_bits(valid, n, lane >> 4);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (!((valid >> v_key(n, lane >> 4, j)) & 1)) v[n][j] = VWord{};
+        if (!((mine >> (j < 4 ? j : 12 + j)) & 1)) v[n][j] = VWord{};
       }
     }
   }

@@ -12,16 +12,13 @@
 // whatever the lengths are, and nothing about them has to be known on the host, so that a captured graph stays
 // valid while they grow.  Every wave finds the line's length and the workgroup's place in it from the lengths
 // themselves (a scan over 64 of them per step).  A workgroup that holds all units of a triple writes its output;
-// otherwise it leaves (o, m, l) in the workspace and join_parts_kernel adds the parts up, in the line's order, so
-// that the result does not depend on timing.
+// otherwise it leaves (o, m, l) in the workspace and takes a ticket of the triple; whoever takes the last one adds
+// the parts up, in the line's order, so that the result does not depend on timing, and resets the tickets.  Nobody waits.
 #pragma once
 
 #include "attn_direct.hpp"
 #include "serving_index.hpp"
 
-#ifndef FLASH_DW
-#define FLASH_DW 2
-#endif
 namespace flash_hip {
 namespace paged {
 
@@ -29,6 +26,7 @@ using namespace direct;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
+constexpr int kMostWorkgroups = 768;  // three to each of 256 compute units
 
 struct Params {
   const char* q;
@@ -40,8 +38,9 @@ struct Params {
   const int32_t* lens;
   const float* k_scale;  // per K/V head, null: 1
   const float* v_scale;
-  float* part_o;         // [2 * workgroups][rows][D]
-  float* part_ml;        // [2 * workgroups][rows][2]
+  float* part_o;         // [2 * workgroups][16 * NQ][D]
+  float* part_ml;        // [2 * workgroups][16 * NQ][2]
+  uint32_t* tickets;     // one for each triple; zero, and left zero
   int64_t q_batch, q_head, o_batch, o_head;     // bytes
   Pages pages;                                   // K and V alike
   int64_t head_stride;                           // bytes
@@ -62,31 +61,34 @@ constexpr int kUnit = kWaves * 32 * kSub<D, CACHE8>;
 __device__ __forceinline__ int32_t length_of(const Params& p, int32_t b) { return cache_length(p.pages, p.lens[b]); }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
-// units of all sequences, and of those before sequence `upto`
-struct Line {
-  uint32_t total, before;
-};
-__device__ __forceinline__ Line measure_line(const Params& p, int32_t unit, int32_t upto, int lane) {
-  Line r{0, 0};
-  for (int32_t b0 = 0; b0 < p.batch; b0 += 64) {
-    const int32_t b = b0 + lane;
-    const uint32_t u = b < p.batch ? units_of(length_of(p, b), unit) : 0u;
-    const uint32_t sum = wave_scan(u);
-    if (upto >= b0 && upto < b0 + 64) r.before = r.total + uniform((uint32_t)__shfl((int)(sum - u), upto - b0));
-    r.total += uniform((uint32_t)__shfl((int)sum, 63));
-  }
-  return r;
+// K and V are read once: without a place in the caches a large read runs at 6.4-6.6 TB/s on this chip, with one at 5.7-5.9
+// (512 MB and 1 GB, 8 and 16 KB of every wave in flight, in order or not).
+template <typename T>
+__device__ __forceinline__ T stream(const T* p) {
+  return __builtin_nontemporal_load(p);
 }
 
 template <int D, int EK, bool CACHE8, int NQ, bool FULL, bool PAGE16>
-__global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params p) {
+__global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NS = kSub<D, CACHE8>;
   constexpr int kUnitKeys = kUnit<D, CACHE8>;
   using S = Step<D, EK, CACHE8, NS, NQ>;
-  constexpr int kRowFloats = D + 4;  // rows of the join buffer, shifted by four banks each
-  __shared__ __attribute__((aligned(16))) float sh_o[kWaves][16][kRowFloats];
+  constexpr int kRowFloats = D + 4;  // rows of the waves' sums, shifted by four banks each
+  // the waves' sums; later the weights of a triple's parts (at most `workgroups` of them, for 8 rows)
+  constexpr int kShFloats = kWaves * 16 * kRowFloats > 8 * kMostWorkgroups ? kWaves * 16 * kRowFloats : 8 * kMostWorkgroups;
+  __shared__ __attribute__((aligned(16))) float sh[kShFloats];
+  __shared__ __attribute__((aligned(16))) f32x4 sh_sum[kThreads];
   __shared__ float sh_ml[kWaves][NQ * 16][2];
+  __shared__ float sh_l[8];
+  __shared__ uint32_t sh_ticket;
+  float(&sh_o)[kWaves][16][kRowFloats] = *(float(*)[kWaves][16][kRowFloats]) & sh[0];
+
+  // Parts go to memory and come from there past the L2s, which the XCDs do not share (sc0 sc1: system scope).  A release
+  // and an acquire at agent scope write back and drop whole L2s instead: 174 us where this takes 66 (32 ragged sequences).
+  constexpr int kThrough = 17;
+  const __amdgpu_buffer_rsrc_t part_o = __builtin_amdgcn_make_buffer_rsrc(p.part_o, 0, (int)(p.workgroups * 2u * 16u * NQ * D * 4u), 0x00020000);
+  const __amdgpu_buffer_rsrc_t part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, (int)(p.workgroups * 2u * 16u * NQ * 8u), 0x00020000);
 
   const int lane = threadIdx.x & 63;
   const int wave = (int)uniform(threadIdx.x >> 6);
@@ -94,24 +96,30 @@ __global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params
 
   // ---- this workgroup's piece of the line -------------------------------------------------------------
   const uint32_t vheads = (uint32_t)(p.kv_heads * p.qblocks);
-  const uint32_t total = measure_line(p, kUnitKeys, -1, lane).total * vheads;
+  auto units_at = [&](int32_t b0) __attribute__((always_inline)) {
+    return b0 + lane < p.batch ? units_of(length_of(p, b0 + lane), kUnitKeys) * vheads : 0u;
+  };
+  uint32_t own = units_at(0), sum = wave_scan(own);
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  for (int32_t b0 = 64; b0 < p.batch; b0 += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_at(b0)), 63);
   const uint32_t c = units_each(total, p.workgroups);
   const uint32_t r_begin = blockIdx.x * c;
   if (r_begin >= total) return;
   const uint32_t r_end = r_begin + c < total ? r_begin + c : total;
   int32_t b = 0;
   uint32_t first = 0;  // units of the line before sequence b
-  for (int32_t b0 = 0; b0 < p.batch; b0 += 64) {
-    const uint32_t u = b0 + lane < p.batch ? units_of(length_of(p, b0 + lane), kUnitKeys) * vheads : 0u;
-    const uint32_t sum = wave_scan(u);
+  for (int32_t b0 = 0;;) {
     const uint64_t past = __builtin_amdgcn_ballot_w64(first + sum > r_begin);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       b = b0 + at;
-      first += uniform((uint32_t)__shfl((int)(sum - u), at));
+      first += (uint32_t)__builtin_amdgcn_readlane((int)(sum - own), at);
       break;
     }
-    first += uniform((uint32_t)__shfl((int)sum, 63));
+    first += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    b0 += 64;
+    own = units_at(b0);
+    sum = wave_scan(own);
   }
   int32_t len = (int32_t)uniform((uint32_t)length_of(p, b));
   uint32_t units = units_of(len, kUnitKeys);
@@ -164,16 +172,24 @@ __global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params
       const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), 16 * t);
       return (int64_t)(((uint64_t)hi << 32) | lo);
     };
+    // (offsets inside a page, opaque so that they stay 32-bit registers beside a scalar base)
+    uint32_t k_row = (uint32_t)n * slot_stride, v_row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v_row[j] = (uint32_t)(4 * g + j) * slot_stride + (FULL || n * S::kE < p.d ? (uint32_t)(n * S::kE * S::kElem) : 0u);
     auto load_k = [&](typename S::KBlock& k, int64_t at) __attribute__((always_inline)) {
+      if constexpr (PAGE16) asm volatile("" : "+v"(k_row));
 #pragma unroll
       for (int t = 0; t < 2 * NS; ++t) {
         const char* src = PAGE16 ? kh + tile_start(at, t) : kh + __shfl(at, 16 * t + n);
-        const uint32_t row = PAGE16 ? (uint32_t)n * slot_stride : 0u;
 #pragma unroll
         for (int i = 0; i < S::kKLoads; ++i) {
           const int col = S::load_column(i, g);
           const bool in = FULL || col < p.d;
-          k[t][i] = *(const u32x4*)(src + (row + (uint32_t)((in ? col : 0) * S::kElem)));
+          if constexpr (PAGE16 && FULL) {
+            k[t][i] = stream((const u32x4*)(src + (k_row + (uint32_t)(S::load_column(0, g) * S::kElem)) + S::load_column(i, 0) * S::kElem));
+          } else {
+            k[t][i] = stream((const u32x4*)(src + ((PAGE16 ? k_row : 0u) + (uint32_t)((in ? col : 0) * S::kElem))));
+          }
           if constexpr (!FULL) {
             // (an 8-bit load holds 16 columns, of which the last 8 may lie behind the row)
             if (!in) k[t][i] = u32x4{0u, 0u, 0u, 0u};
@@ -185,55 +201,39 @@ __global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params
       }
     };
     auto load_v = [&](typename S::VBlock& v, int64_t at) __attribute__((always_inline)) {
-      const bool in = FULL || n * S::kE < p.d;
-      const uint32_t col = (uint32_t)(in ? n * S::kE * S::kElem : 0);
+      if constexpr (PAGE16) asm volatile("" : "+v"(v_row[0]), "+v"(v_row[1]), "+v"(v_row[2]), "+v"(v_row[3]));
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if constexpr (PAGE16) {
-            const uint32_t row = (uint32_t)(4 * g + j % 4) * slot_stride;
-            v[s][j] = *(const typename S::VWord*)(vv + tile_start(at, 2 * s + j / 4) + (row + col));
+            v[s][j] = stream((const typename S::VWord*)(vv + tile_start(at, 2 * s + j / 4) + v_row[j % 4]));
           } else {
-            v[s][j] = *(const typename S::VWord*)(vv + __shfl(at, S::v_key(s, g, j)) + col);
+            v[s][j] = stream((const typename S::VWord*)(vv + __shfl(at, S::v_key(s, g, j)) + (FULL || n * S::kE < p.d ? n * S::kE * S::kElem : 0)));
           }
         }
       }
     };
 
-    // K is fetched a step ahead, V at the step's beginning: 16 KB in flight per wave at any time at d = 128
+    // A step's K and V are fetched together at its beginning, the pages' entries a step ahead: 16 KB in flight per wave at
+    // d = 128, and the registers leave room for three waves on a SIMD.
     typename S::State st;
     auto attend = [&](auto careful) __attribute__((always_inline)) {
       S::clear(st);
-      typename S::KBlock k, k_next;
-      int64_t at, at_next;
-      uint64_t valid = place(u0, page_of(u0), at), valid_next;
-      int32_t page = page_of(u0 + 1);
-      load_k(k, at);
+      int32_t page = page_of(u0);
       for (uint32_t u = u0; u < u1; ++u) {
+        typename S::KBlock k;
         typename S::VBlock v;
+        int64_t at;
+        const uint64_t valid = place(u, page, at);
+        page = page_of(u + 1);
+        if (valid == 0) continue;
+        load_k(k, at);
         load_v(v, at);
-        const bool more = u + 1 < u1;
-        if (more) {
-          valid_next = place(u + 1, page, at_next);
-          load_k(k_next, at_next);
-          page = page_of(u + 2);
-        }
-        if (valid != 0) {
-          typename S::Weights w;
-          S::template weigh<false>(st, w, k, qf, valid, sc, lane);
-          S::clear_missing(v, valid, lane);
-          S::template accumulate<decltype(careful)::value>(st, w, v);
-        }
-        if (more) {
-#pragma unroll
-          for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-            for (int i = 0; i < S::kKLoads; ++i) k[t][i] = k_next[t][i];
-          }
-          at = at_next;
-          valid = valid_next;
-        }
+        typename S::Weights w;
+        S::template weigh<false>(st, w, k, qf, valid, sc, lane);
+        S::clear_missing(v, valid, lane);
+        S::template accumulate<decltype(careful)::value>(st, w, v);
       }
     };
     attend(std::false_type{});
@@ -288,13 +288,89 @@ __global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params
               p.lse[(int64_t)b * p.kv_heads * p.group + head] = l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
             }
           } else {
-            const uint64_t at = (uint64_t)slot * (16 * NQ) + (uint32_t)(16 * q + row);
-            *(f32x4*)(p.part_o + at * D + col) = sum;
-            if (col == 0) *(f32x2*)(p.part_ml + at * 2) = f32x2{m, l};
+            const uint32_t at = slot * (16 * NQ) + (uint32_t)(16 * q + row);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), part_o, (at * D + (uint32_t)col) * 4u, 0, kThrough);
+            if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, part_ml, at * 8u, 0, kThrough);
           }
         }
       }
       __syncthreads();
+    }
+
+    // ---- the last workgroup of a triple to come here adds its parts up, in the line's order
+    if (!complete) {
+      const uint32_t start = r - u0, w0 = start / c, parts = (start + units - 1) / c - w0 + 1;
+      uint32_t* const ticket = p.tickets + ((uint32_t)b * vheads + vh);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the part has reached memory
+      __syncthreads();
+      if (threadIdx.x == 0) sh_ticket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (sh_ticket == parts - 1) {
+        asm volatile("" ::: "memory");
+        if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        auto row_of = [&](uint32_t i, int row) __attribute__((always_inline)) { return part_slot(w0 + i, c, start) * (16 * NQ) + (uint32_t)row; };
+#pragma unroll 1
+        for (int q = 0; 8 * q < rows; ++q) {
+          // weights of the parts: 32 lanes for each of 8 rows
+          const int row = threadIdx.x / 32, sub = threadIdx.x % 32;
+          const bool there = 8 * q + row < rows;
+          float m = kMinusInf;
+          for (uint32_t i = sub; there && i < parts; i += 32) {
+            const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part_ml, row_of(i, 8 * q + row) * 8u, 0, kThrough));
+            sh[row * kMostWorkgroups + i] = x;
+            m = fmaxf(m, x);
+          }
+#pragma unroll
+          for (int s = 1; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
+          const float ref = m == kMinusInf ? 0.f : m;
+          float l = 0.f;
+          for (uint32_t i = sub; there && i < parts; i += 32) {
+            const float f = __builtin_amdgcn_exp2f(sh[row * kMostWorkgroups + i] - ref);
+            sh[row * kMostWorkgroups + i] = f;
+            l += f * __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part_ml, row_of(i, 8 * q + row) * 8u + 4u, 0, kThrough));
+          }
+#pragma unroll
+          for (int s = 1; s < 32; s <<= 1) l += __shfl_xor(l, s);
+          if (there && sub == 0) {
+            sh_l[row] = l;
+            if (p.lse) {
+              p.lse[(int64_t)b * p.kv_heads * p.group + kvh * p.group + row0 + 8 * q + row] =
+                  l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
+            }
+          }
+          __syncthreads();
+          // the sums: four columns a thread, the parts dealt to `sides` groups of threads where there are few rows
+          constexpr int kPieces = D / 4;
+          const int here = rows - 8 * q < 8 ? rows - 8 * q : 8, items = here * kPieces;
+          const int sides = items >= kThreads ? 1 : kThreads / items;
+          for (int x0 = 0; x0 < items; x0 += kThreads) {
+            const int x = sides == 1 ? x0 + (int)threadIdx.x : (int)threadIdx.x % items, side = sides == 1 ? 0 : (int)threadIdx.x / items;
+            const int r8 = x / kPieces, col = 4 * (x % kPieces);
+            const bool mine = x < items && side < sides && col < p.d;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            if (mine) {
+#pragma unroll 4
+              for (uint32_t i = (uint32_t)side; i < parts; i += (uint32_t)sides) {
+                acc += sh[r8 * kMostWorkgroups + i] *
+                       __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part_o, (row_of(i, 8 * q + r8) * D + (uint32_t)col) * 4u, 0, kThrough));
+              }
+            }
+            if (sides > 1) {
+              sh_sum[threadIdx.x] = acc;
+              __syncthreads();
+              if (mine && side == 0) {
+                for (int s = 1; s < sides; ++s) acc += sh_sum[s * items + x];
+              }
+            }
+            if (mine && side == 0) {
+              const float inv = sh_l[r8] == 0.f ? 0.f : vs / sh_l[r8];
+              *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)(kvh * p.group + row0 + 8 * q + r8) * p.o_head + col * 2) =
+                  u32x2{pack2<EK>(acc[0] * inv, acc[1] * inv), pack2<EK>(acc[2] * inv, acc[3] * inv)};
+            }
+          }
+          __syncthreads();
+        }
+      }
     }
 
     // ---- the next triple of the line ---------------------------------------------------------------------
@@ -308,66 +384,6 @@ __global__ __launch_bounds__(kThreads, FLASH_DW) void decode_kernel(const Params
         units = units_of(len, kUnitKeys);
       }
     }
-  }
-#endif
-}
-
-// One workgroup per sequence and query head: the parts of its triple, if there are several, in the line's order.
-// 32 lanes (16 at D = 64) hold a row, the others other parts of it.
-template <int D, int EK, bool CACHE8, int NQ>
-__global__ __launch_bounds__(kThreads) void join_parts_kernel(const Params p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int kPieces = D / 4, kSides = kThreads / kPieces;
-  __shared__ __attribute__((aligned(16))) float sh_o[kSides][D];
-  __shared__ float sh_ml[kSides][2];
-  const int lane = threadIdx.x & 63;
-  const int32_t heads = p.kv_heads * p.group;
-  const int32_t b = (int32_t)(blockIdx.x / (uint32_t)heads), head = (int32_t)blockIdx.x - b * heads;
-  const int32_t kvh = head / p.group, in_group = head - kvh * p.group;
-  const uint32_t vheads = (uint32_t)(p.kv_heads * p.qblocks);
-  constexpr int kUnitKeys = kUnit<D, CACHE8>;
-  const Line line = measure_line(p, kUnitKeys, b, lane);
-  const uint32_t units = units_of((int32_t)uniform((uint32_t)length_of(p, b)), kUnitKeys);
-  const uint32_t c = units_each(line.total * vheads, p.workgroups);
-  const uint32_t start = line.before * vheads + (uint32_t)(kvh * p.qblocks + in_group / (16 * NQ)) * units;
-  const uint32_t w0 = start / c, w1 = (start + units - 1) / c;
-  if (w0 == w1) return;  // one workgroup had it all and wrote the output
-  const int side = threadIdx.x / kPieces, col = 4 * (threadIdx.x % kPieces);
-  float m = kMinusInf, l = 0.f;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t w = w0 + (uint32_t)side; w <= w1; w += kSides) {
-    const uint32_t slot = part_slot(w, c, start);
-    const uint64_t at = (uint64_t)slot * (16 * NQ) + (uint32_t)(in_group % (16 * NQ));
-    const f32x2 ml = *(const f32x2*)(p.part_ml + at * 2);
-    const f32x4 x = col < p.d ? *(const f32x4*)(p.part_o + at * D + col) : f32x4{0.f, 0.f, 0.f, 0.f};
-    const float m_new = fmaxf(m, ml[0]), ref = m_new == kMinusInf ? 0.f : m_new;
-    const float keep = __builtin_amdgcn_exp2f(m - ref), add = __builtin_amdgcn_exp2f(ml[0] - ref);
-    sum = sum * keep + x * add;
-    l = l * keep + ml[1] * add;
-    m = m_new;
-  }
-  *(f32x4*)&sh_o[side][col] = sum;
-  if (col == 0) {
-    sh_ml[side][0] = m;
-    sh_ml[side][1] = l;
-  }
-  __syncthreads();
-  if (side == 0 && col < p.d) {
-#pragma unroll
-    for (int s = 1; s < kSides; ++s) m = fmaxf(m, sh_ml[s][0]);
-    const float ref = m == kMinusInf ? 0.f : m;
-    l = 0.f;
-    sum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < kSides; ++s) {
-      const float f = __builtin_amdgcn_exp2f(sh_ml[s][0] - ref);
-      l += f * sh_ml[s][1];
-      sum += f * *(const f32x4*)&sh_o[s][col];
-    }
-    const float inv = l == 0.f ? 0.f : (CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f) / l;
-    *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)head * p.o_head + col * 2) =
-        u32x2{pack2<EK>(sum[0] * inv, sum[1] * inv), pack2<EK>(sum[2] * inv, sum[3] * inv)};
-    if (p.lse && col == 0) p.lse[(int64_t)b * heads + head] = l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
   }
 #endif
 }

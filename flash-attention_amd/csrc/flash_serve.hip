@@ -99,15 +99,16 @@ flash_hip::Pages pages_of(const flash_paged_cache* c, int64_t elem) {
 // ---- decoding ---------------------------------------------------------------------------------------------------
 using DecodeParams = flash_hip::paged::Params;
 
-// Two workgroups of four waves on each of 256 compute units hold the registers of two steps of K and V per wave
-// (128 KB in flight per compute unit); with 64 query rows one fits.
-constexpr uint32_t kDecodeWorkgroups = 512;
+constexpr uint32_t kDecodeWorkgroups = flash_hip::paged::kMostWorkgroups;
+// Workspace: room for two parts of every workgroup at the largest tile, then a ticket for each triple.  The tickets' place
+// does not depend on the shape: parts of one call never lie where another call looks for zeros.
+constexpr int64_t kPartRows = (int64_t)2 * kDecodeWorkgroups * 16, kPartBytes = kPartRows * (128 * 4 + 8);
+static_assert(kPartBytes == FLASH_DECODE_PARTS_BYTES, "include/flash_hip.h names the part of the workspace that need not be zero");
 
 struct DecodePlan {
   int tile_d, nq;
   uint32_t workgroups;
-  bool join;              // some sequence may be cut
-  int64_t part_o_bytes, bytes;
+  int64_t bytes;  // 0: no sequence can be cut
 };
 int plan_decode(const flash_decode_args* a, const flash_paged_cache* c, bool memory, DecodePlan* plan) {
   REFUSE_IF(!a, "null flash_decode_args");
@@ -126,30 +127,23 @@ int plan_decode(const flash_decode_args* a, const flash_paged_cache* c, bool mem
   const int64_t most = reach <= unit ? 1 : (reach + unit - 1) / unit;  // units of a sequence
   const int64_t triples = c->sequences * c->kv_heads * ((group + 16 * plan->nq - 1) / (16 * plan->nq));
   REFUSE_IF(triples * most >= (int64_t)1 << 31 || c->sequences * a->q_heads >= (int64_t)1 << 31, "batch of %lld sequences is too large", (long long)c->sequences);
-  const int64_t limit = plan->nq == 4 ? kDecodeWorkgroups / 2 : kDecodeWorkgroups;
-  plan->workgroups = (uint32_t)(triples * most < limit ? triples * most : limit);
-  plan->join = most > 1;
-  const int64_t rows = plan->join ? (int64_t)2 * plan->workgroups * 16 * plan->nq : 0;
-  plan->part_o_bytes = rows * plan->tile_d * 4;
-  plan->bytes = plan->part_o_bytes + rows * 8;
+  plan->workgroups = (uint32_t)(triples * most < kDecodeWorkgroups ? triples * most : kDecodeWorkgroups);
+  plan->bytes = most > 1 && triples > 0 ? kPartBytes + (triples * 4 + 15) / 16 * 16 : 0;
   return FLASH_HIP_OK;
 }
 
 template <int D, int EK, bool CACHE8, int NQ>
-int launch_decode(const DecodeParams& p, bool join, hipStream_t stream) {
+int launch_decode(const DecodeParams& p, hipStream_t stream) {
   namespace pg = flash_hip::paged;
   const bool page16 = p.pages.page_shift >= 4 && 16 * p.pages.slot_stride < ((int64_t)1 << 31);
   auto kernel = p.d == D ? (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, true, true> : pg::decode_kernel<D, EK, CACHE8, NQ, true, false>)
                          : (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, false, true> : pg::decode_kernel<D, EK, CACHE8, NQ, false, false>);
   hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(pg::kThreads), 0, stream, p);
-  CHECK(launched("flash_decode_paged"));
-  if (!join) return FLASH_HIP_OK;
-  hipLaunchKernelGGL((pg::join_parts_kernel<D, EK, CACHE8, NQ>), dim3((uint32_t)(p.batch * p.kv_heads * p.group)), dim3(pg::kThreads), 0, stream, p);
   return launched("flash_decode_paged");
 }
 template <int D, int EK, bool CACHE8>
 int launch_decode(const DecodeParams& p, const DecodePlan& plan, hipStream_t stream) {
-  return launch_decode<D, EK, CACHE8, 1>(p, plan.join, stream);
+  return launch_decode<D, EK, CACHE8, 1>(p, stream);
 }
 template <int D>
 int launch_decode(const DecodeParams& p, const DecodePlan& plan, int dtype, bool cache8, hipStream_t stream) {
@@ -200,7 +194,8 @@ int flash_decode_paged(const flash_decode_args* a, const flash_paged_cache* c, v
   p.k_scale = c->k_scale;
   p.v_scale = c->v_scale;
   p.part_o = (float*)workspace;
-  p.part_ml = (float*)((char*)workspace + plan.part_o_bytes);
+  p.part_ml = p.part_o + kPartRows * 128;
+  p.tickets = (uint32_t*)((char*)workspace + kPartBytes);
   p.q_batch = a->q_batch_stride * 2;
   p.q_head = a->q_head_stride * 2;
   p.o_batch = a->o_batch_stride * 2;

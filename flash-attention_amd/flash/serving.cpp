@@ -6,6 +6,8 @@
 #include <hip/hip_runtime_api.h>
 
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <sstream>
 #include <stdexcept>
 
@@ -67,6 +69,30 @@ const Tensor& or_none(const Maybe& t) { return t ? *t : kNone; }
 void wait_for(const c10::hip::HIPStreamMasqueradingAsCUDA& stream) {
   const hipError_t e = hipStreamSynchronize(stream.stream());
   if (e != hipSuccess) throw std::runtime_error(hipGetErrorString(e));
+}
+
+// Zero-filled scratch for flash_decode_paged.  Work on one stream runs in order, so its calls share a buffer that is
+// filled once, on their first call (and again when a larger one is needed).  A graph under capture gets one of its own,
+// filled by a node of the graph: it may be replayed on any stream, beside any other.  So does a call on a stream that torch
+// did not make, whose handle may come to stand for another stream.
+Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradingAsCUDA& stream, int64_t need) {
+  const auto options = at::TensorOptions().dtype(at::kByte).device(device);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess) throw std::runtime_error("hipStreamIsCapturing failed");
+  const c10::StreamId id = stream.unwrap().id();
+  const bool own_stream = id == 0 || (id & 1) != 0;  // torch's numbering: the default stream, and the streams of its pools
+  auto fresh = [&](int64_t bytes) {
+    Tensor t = at::empty({bytes}, options);
+    t.narrow(0, FLASH_DECODE_PARTS_BYTES, bytes - FLASH_DECODE_PARTS_BYTES).zero_();
+    return t;
+  };
+  if (capture != hipStreamCaptureStatusNone || !own_stream) return fresh(need);
+  static std::mutex mutex;
+  static auto& buffers = *new std::map<std::pair<int, c10::StreamId>, Tensor>;  // (never destroyed: the allocator may be gone by then)
+  const std::lock_guard<std::mutex> lock(mutex);
+  Tensor& t = buffers[{device.index(), id}];
+  if (!t.defined() || t.numel() < need) t = fresh(need + (1 << 16));
+  return t;
 }
 
 flash_paged_cache describe(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor* lens, const Tensor& k_scale, const Tensor& v_scale) {
@@ -221,14 +247,9 @@ std::tuple<Tensor, Tensor> decode_paged(const Tensor& q, const Tensor& k_cache, 
     lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
     a.lse = static_cast<float*>(lse.data_ptr());
   }
-  void* ws = nullptr;
-  if (need > 0) {
-    // from the allocator, which hands the block out again in stream order (inside a capture: from the graph's own pool)
-    scratch = workspace ? *workspace : torch::empty({need}, q.options().dtype(at::kByte).requires_grad(false));
-    ws = scratch.data_ptr();
-  }
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
-  raise(flash_decode_paged(&a, &c, ws, need, stream.stream()));
+  if (need > 0) scratch = workspace ? *workspace : stream_workspace(q.device(), stream, need);
+  raise(flash_decode_paged(&a, &c, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
   if (sync) wait_for(stream);
   return {o, lse};
 }

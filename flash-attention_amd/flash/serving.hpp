@@ -24,8 +24,8 @@ torch::Tensor forward_packed(const torch::Tensor& q, const torch::Tensor& k, con
 
 // q [sequences, Hq, d]; caches [pages, Hkv, page_size, d]; page_table int32 [sequences, width]; seq_lens int32
 // [sequences].  Returns the output and, when asked for, the logarithm of the weights' sum (float32 [sequences, Hq]; an
-// undefined tensor otherwise).  `workspace`: at least decode_workspace_bytes bytes; absent, it comes from torch's
-// allocator.
+// undefined tensor otherwise).  `workspace`: at least decode_workspace_bytes bytes, zero-filled before its first use; absent,
+// calls on one of torch's streams share one that is kept for it, and every captured graph has its own.
 std::tuple<torch::Tensor, torch::Tensor> decode_paged(
     const torch::Tensor& q, const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& page_table,
     const torch::Tensor& seq_lens, std::optional<double> softmax_scale, const std::optional<torch::Tensor>& k_scale,

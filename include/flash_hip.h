@@ -287,9 +287,10 @@ typedef struct flash_paged_cache {
  * Attention of one new token of every sequence over the cache: q [sequences, q_heads, d] (16-bit, dtype), whose key
  * and value are in the cache already.  lse (may be NULL): [sequences, q_heads], contiguous, the natural logarithm of
  * the sum of the weights exp(softmax_scale q.k).  A sequence of length 0 gets zeros and -inf.
- * `workspace`: device memory, 16-byte aligned, flash_decode_paged_workspace_bytes(...) bytes; scratch, not to be
- * touched until the call's work has finished, nor shared by calls that may overlap in time (two captured graphs
- * among them).
+ * `workspace`: device memory, 16-byte aligned, flash_decode_paged_workspace_bytes(...) bytes, filled with zeros before its
+ * first use (what lies behind its first FLASH_DECODE_PARTS_BYTES; the rest may hold anything).  Every call leaves the part of it that has to be zero as it found it, so it serves any number of calls, of any
+ * shape, one after the other; it is not to be touched until a call's work has finished, nor shared by calls that may
+ * overlap in time (two captured graphs among them).
  */
 typedef struct flash_decode_args {
   const void* q;
@@ -300,6 +301,7 @@ typedef struct flash_decode_args {
   float softmax_scale;
   int32_t dtype;                 /* of q and o; a 16-bit cache has the same */
 } flash_decode_args;
+#define FLASH_DECODE_PARTS_BYTES (2ll * 768 * 16 * (128 * 4 + 8))
 int flash_decode_paged(const flash_decode_args* args, const flash_paged_cache* cache, void* workspace,
                        int64_t workspace_bytes, void* hip_stream);
 /* -1 (and an error text) for what flash_decode_paged refuses.  Looks at sizes only; does not touch the GPU. */

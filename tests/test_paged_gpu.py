@@ -167,12 +167,53 @@ def test_decode_output_workspace_and_strides(fa):
     want = fa.decode_paged(qd, *caches, tab, n)
     check_decode(want, None, q, rows, lens, d ** -0.5)
     need = fa.decode_workspace_bytes(qd, caches[0], tab)
-    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")     # (its contents do not matter: these are NaN)
-    room = torch.full((2, 9, d), 3.0, dtype=BF16, device="cuda")
-    got = fa.decode_paged(qd, *caches, tab, n, out=room[:, :8], workspace=ws)
-    assert torch.equal(got, want) and bool((room[:, 8] == 3.0).all())
+    ws = fa.decode_workspace(qd, caches[0], tab)
+    assert ws.numel() == need > 0
+    for _ in range(3):                                        # one workspace for any number of calls
+        room = torch.full((2, 9, d), 3.0, dtype=BF16, device="cuda")
+        got = fa.decode_paged(qd, *caches, tab, n, out=room[:, :8], workspace=ws)
+        assert torch.equal(got, want) and bool((room[:, 8] == 3.0).all())
     with pytest.raises(ValueError, match="workspace"):
         fa.decode_paged(qd, *caches, tab, n, workspace=ws[:need // 2])
+
+
+def test_one_workspace_for_calls_of_different_shapes(fa):
+    """Shapes, head dims and cut lengths by turns on one workspace and on the stream's own."""
+    ws = None
+    calls = []
+    for lens, page, hq, hk, d, dtype in (([5000], 16, 8, 2, 128, F16), ([300] * 40, 32, 4, 4, 64, BF16), ([900, 2, 4000], 64, 16, 1, 96, F16),
+                                         ([1300] * 9, 16, 20, 2, 128, BF16)):
+        kc, vc, table, rows = filled(lens, page, hk, d, dtype, seed=sum(lens))
+        q = torch.randn(len(lens), hq, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+        args = (q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+        mine = fa.decode_workspace(args[0], args[1], args[3])
+        if ws is None or mine.numel() > ws.numel():
+            ws = mine
+        calls.append((args, q, rows, lens, d))
+    for _ in range(2):
+        for args, q, rows, lens, d in calls + calls[::-1]:
+            got = fa.decode_paged(*args, workspace=ws)
+            assert torch.equal(got, fa.decode_paged(*args))
+    for args, q, rows, lens, d in calls:
+        check_decode(fa.decode_paged(*args), None, q, rows, lens, d ** -0.5, heads=[0, q.shape[1] - 1])
+
+
+def test_streams_decode_side_by_side(fa):
+    """The same call on several streams at once: scratch is kept for each of them."""
+    lens = [3000, 1200, 40]
+    kc, vc, table, _ = filled(lens, 16, 2, 128, F16, seed=33)
+    q = torch.randn(3, 4, 128, generator=torch.Generator().manual_seed(1)).half().cuda()
+    args = (q, kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    want = fa.decode_paged(*args)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(fa.decode_paged(*args, sync=False))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
 
 
 def test_parts_join_through_lse(fa):

@@ -126,12 +126,13 @@ def test_append_refusals(fa, change, match):
 
 
 def test_workspace_query(fa):
-    """No scratch where no sequence can be cut; otherwise two parts for each of at most 512 workgroups."""
+    """No scratch where no sequence can be cut; otherwise two parts for each of at most 768 workgroups at the largest head
+    dim, and a ticket for each sequence and K/V head."""
     a = paged()
     assert fa.decode_workspace_bytes(a["q"], a["k_cache"], a["page_table"]) == 0
     wide = torch.zeros(2, 4096, dtype=torch.int32)
     need = fa.decode_workspace_bytes(a["q"], a["k_cache"], wide)
-    assert need == 2 * 512 * 16 * (64 * 4 + 8)
+    assert need == 2 * 768 * 16 * (128 * 4 + 8) + 16
     assert fa.decode_workspace_bytes(a["q"], a["k_cache"], torch.zeros(2, 1 << 22, dtype=torch.int32)) == need
 
 
