@@ -264,9 +264,9 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
       }
       __syncthreads();
       constexpr int kPieces = D / 4;
-      for (int x = threadIdx.x; x < 16 * kPieces; x += kThreads) {
+      for (int x = threadIdx.x; x < 16 * kPieces && 16 * q + x / kPieces < rows; x += kThreads) {
         const int row = x / kPieces, col = 4 * (x % kPieces);
-        if (16 * q + row < rows && col < p.d) {
+        if (col < p.d) {
           float m = kMinusInf;
 #pragma unroll
           for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sh_ml[w][16 * q + row][0]);
@@ -309,66 +309,88 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
         asm volatile("" ::: "memory");
         if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         auto row_of = [&](uint32_t i, int row) __attribute__((always_inline)) { return part_slot(w0 + i, c, start) * (16 * NQ) + (uint32_t)row; };
-#pragma unroll 1
-        for (int q = 0; 8 * q < rows; ++q) {
+        // Loads past the caches take two microseconds: all of them go out together, the first ones of the sums even before
+        // the weights are known.  Sums: four columns a thread; with few rows the parts are dealt to `sides` groups of
+        // threads, TOGETHER parts a thread at a time.  (Indexes behind the last part read it again.)
+        auto join_rows = [&](int q, auto together_tag, auto more_tag) __attribute__((always_inline)) {
+          constexpr int kPieces = D / 4, kTogether = decltype(together_tag)::value, kMore = decltype(more_tag)::value;
+          const int here = rows - 8 * q < 8 ? rows - 8 * q : 8, items = here * kPieces, sides = kThreads / items;
+          const int x = (int)threadIdx.x % items, side = (int)threadIdx.x / items, r8 = x / kPieces, col = 4 * (x % kPieces);
+          f32x4 part[kTogether];
+          auto fetch = [&](uint32_t i0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+              const uint32_t i = i0 + (uint32_t)(k * sides);
+              part[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      part_o, (row_of(i < parts ? i : parts - 1, 8 * q + r8) * D + (uint32_t)col) * 4u, 0, kThrough));
+            }
+          };
+          fetch((uint32_t)side);
           // weights of the parts: 32 lanes for each of 8 rows
           const int row = threadIdx.x / 32, sub = threadIdx.x % 32;
           const bool there = 8 * q + row < rows;
-          float m = kMinusInf;
-          for (uint32_t i = sub; there && i < parts; i += 32) {
-            const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part_ml, row_of(i, 8 * q + row) * 8u, 0, kThrough));
-            sh[row * kMostWorkgroups + i] = x;
-            m = fmaxf(m, x);
-          }
+          float m = kMinusInf, l = 0.f;
+          for (uint32_t i0 = sub; i0 < parts; i0 += 32 * kMore) {
+            u32x2 ml[kMore];
 #pragma unroll
-          for (int s = 1; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
-          const float ref = m == kMinusInf ? 0.f : m;
-          float l = 0.f;
-          for (uint32_t i = sub; there && i < parts; i += 32) {
-            const float f = __builtin_amdgcn_exp2f(sh[row * kMostWorkgroups + i] - ref);
-            sh[row * kMostWorkgroups + i] = f;
-            l += f * __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part_ml, row_of(i, 8 * q + row) * 8u + 4u, 0, kThrough));
+            for (int k = 0; k < kMore; ++k) {
+              const uint32_t i = i0 + 32u * (uint32_t)k;
+              ml[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, row_of(i < parts ? i : parts - 1, there ? 8 * q + row : 8 * q) * 8u, 0, kThrough);
+            }
+#pragma unroll
+            for (int k = 0; k < kMore; ++k) {
+              const uint32_t i = i0 + 32u * (uint32_t)k;
+              if (i < parts) {
+                const float mi = __uint_as_float(ml[k][0]), m_new = fmaxf(m, mi), ref = m_new == kMinusInf ? 0.f : m_new;
+                sh[row * kMostWorkgroups + i] = mi;
+                l = l * __builtin_amdgcn_exp2f(m - ref) + __uint_as_float(ml[k][1]) * __builtin_amdgcn_exp2f(mi - ref);
+                m = m_new;
+              }
+            }
           }
+          float top = m;
+#pragma unroll
+          for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+          const float ref = top == kMinusInf ? 0.f : top;
+          l *= __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
           for (int s = 1; s < 32; s <<= 1) l += __shfl_xor(l, s);
+          for (uint32_t i = sub; i < parts; i += 32) sh[row * kMostWorkgroups + i] = __builtin_amdgcn_exp2f(sh[row * kMostWorkgroups + i] - ref);
           if (there && sub == 0) {
             sh_l[row] = l;
             if (p.lse) {
               p.lse[(int64_t)b * p.kv_heads * p.group + kvh * p.group + row0 + 8 * q + row] =
-                  l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
+                  l == 0.f ? kMinusInf : (top + log2f(l)) * 0.693147180559945309f;
             }
           }
           __syncthreads();
-          // the sums: four columns a thread, the parts dealt to `sides` groups of threads where there are few rows
-          constexpr int kPieces = D / 4;
-          const int here = rows - 8 * q < 8 ? rows - 8 * q : 8, items = here * kPieces;
-          const int sides = items >= kThreads ? 1 : kThreads / items;
-          for (int x0 = 0; x0 < items; x0 += kThreads) {
-            const int x = sides == 1 ? x0 + (int)threadIdx.x : (int)threadIdx.x % items, side = sides == 1 ? 0 : (int)threadIdx.x / items;
-            const int r8 = x / kPieces, col = 4 * (x % kPieces);
-            const bool mine = x < items && side < sides && col < p.d;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            if (mine) {
-#pragma unroll 4
-              for (uint32_t i = (uint32_t)side; i < parts; i += (uint32_t)sides) {
-                acc += sh[r8 * kMostWorkgroups + i] *
-                       __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part_o, (row_of(i, 8 * q + r8) * D + (uint32_t)col) * 4u, 0, kThrough));
-              }
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          for (uint32_t i0 = (uint32_t)side; i0 < parts;) {
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+              const uint32_t i = i0 + (uint32_t)(k * sides);
+              if (i < parts) acc += sh[r8 * kMostWorkgroups + i] * part[k];
             }
-            if (sides > 1) {
-              sh_sum[threadIdx.x] = acc;
-              __syncthreads();
-              if (mine && side == 0) {
-                for (int s = 1; s < sides; ++s) acc += sh_sum[s * items + x];
-              }
-            }
-            if (mine && side == 0) {
-              const float inv = sh_l[r8] == 0.f ? 0.f : vs / sh_l[r8];
-              *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)(kvh * p.group + row0 + 8 * q + r8) * p.o_head + col * 2) =
-                  u32x2{pack2<EK>(acc[0] * inv, acc[1] * inv), pack2<EK>(acc[2] * inv, acc[3] * inv)};
-            }
+            i0 += (uint32_t)(kTogether * sides);
+            if (i0 < parts) fetch(i0);
+          }
+          sh_sum[threadIdx.x] = acc;
+          __syncthreads();
+          if (side == 0 && col < p.d) {
+            for (int s = 1; s < sides; ++s) acc += sh_sum[s * items + x];
+            const float inv = sh_l[r8] == 0.f ? 0.f : vs / sh_l[r8];
+            *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)(kvh * p.group + row0 + 8 * q + r8) * p.o_head + col * 2) =
+                u32x2{pack2<EK>(acc[0] * inv, acc[1] * inv), pack2<EK>(acc[2] * inv, acc[3] * inv)};
           }
           __syncthreads();
+        };
+#pragma unroll 1
+        for (int q = 0; 8 * q < rows; ++q) {
+          if (parts <= 8) {
+            join_rows(q, std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+          } else {
+            join_rows(q, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+          }
         }
       }
     }
