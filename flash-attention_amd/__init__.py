@@ -72,7 +72,7 @@ ABI_SYMBOLS = (
     "flash_fwd_f32_workspace_bytes", "flash_fwd_query",
     "flash_fwd_query_entry",
     "flash_kernel_type_name",
-    "flash_fwd_packed", "flash_decode_paged", "flash_decode_paged_workspace_bytes", "flash_cache_append",
+    "flash_fwd_packed", "flash_fwd_packed_workspace_bytes", "flash_decode_paged", "flash_decode_paged_workspace_bytes", "flash_cache_append",
     "flash_hip_last_error", "flash_hip_version", "flash_hip_reload_switches",
 )
 
@@ -106,9 +106,12 @@ def lib() -> ctypes.CDLL:
     L.flash_fwd_query.restype = ctypes.c_int
     L.flash_fwd_query_entry.argtypes = [i64, i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_LaunchInfo)]
     L.flash_fwd_query_entry.restype = ctypes.c_int
-    for name, nargs in (("flash_fwd_packed", 2), ("flash_cache_append", 3)):
-        getattr(L, name).argtypes = [vp] * nargs
-        getattr(L, name).restype = ctypes.c_int
+    L.flash_fwd_packed.argtypes = [vp, vp, i64, vp]
+    L.flash_fwd_packed.restype = ctypes.c_int
+    L.flash_fwd_packed_workspace_bytes.argtypes = [vp]
+    L.flash_fwd_packed_workspace_bytes.restype = i64
+    L.flash_cache_append.argtypes = [vp, vp, vp]
+    L.flash_cache_append.restype = ctypes.c_int
     L.flash_decode_paged.argtypes = [vp, vp, vp, i64, vp]
     L.flash_decode_paged.restype = ctypes.c_int
     L.flash_decode_paged_workspace_bytes.argtypes = [vp, vp]

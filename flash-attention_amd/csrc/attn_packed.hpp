@@ -24,6 +24,11 @@ struct Params {
   int32_t sequences, total_q, total_k, heads, kv_heads, d;
   int32_t causal;
   uint32_t tiles;     // query tiles of the grid, per head
+  uint32_t items;     // workgroups of the grid for one part of every item
+  int32_t parts;      // most parts of an item (1: items are not cut)
+  float* part_o;      // [items * parts][4 waves][query blocks][D / 16][64 lanes][4]
+  float* part_ml;     // [items * parts][rows][2]
+  uint32_t* tickets;  // [items]; zero, and left zero
   float scale_log2;   // softmax scale * log2 e
 };
 
@@ -161,9 +166,11 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
 
 }  // namespace packed
 
-// the pipelined kernel (flash_packed.hip): whether it takes a call, and its launch
+// the pipelined kernel (flash_packed.hip): whether it takes a call, the workspace with which it can cut items (0: it would
+// not), and its launch
 __attribute__((visibility("hidden"))) bool packed_mfma_takes(const packed::Params& p);
-__attribute__((visibility("hidden"))) int launch_packed_mfma(packed::Params p, bool bf16, hipStream_t stream);
+__attribute__((visibility("hidden"))) int64_t packed_mfma_workspace(const packed::Params& p);
+__attribute__((visibility("hidden"))) int launch_packed_mfma(const packed::Params& p, bool bf16, void* workspace, hipStream_t stream);
 
 namespace packed {
 

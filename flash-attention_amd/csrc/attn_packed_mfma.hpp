@@ -62,12 +62,12 @@ struct Item {
   int32_t row0;  // first row inside the sequence, may be negative
   int32_t a0;    // keys seen by all rows of the item, a multiple of 64; negative: some rows see none
 };
-__device__ __forceinline__ Item find_item(const Params& p, int32_t rows, bool causal, int lane) {
+__device__ __forceinline__ Item find_item(const Params& p, uint32_t id, int32_t rows, bool causal, int lane) {
   Item x;
   auto extent = [&](int32_t nq, int32_t nk) __attribute__((always_inline)) { return nq > 0 ? nq + packed_shift(nq, nk, causal) : 0; };
   const TileLine<decltype(extent)> line{p, rows, lane, extent};
   const auto c = line.chunk(0);
-  const ItemPlace at = item_place(blockIdx.x, line.length(c), (uint32_t)p.heads, (uint32_t)p.kv_heads);
+  const ItemPlace at = item_place(id, line.length(c), (uint32_t)p.heads, (uint32_t)p.kv_heads);
   x.it.there = at.there;
   if (!at.there) return x;
   x.head = (int32_t)at.head;

@@ -29,20 +29,40 @@ template <int T>
 using DiagonalPlan = TilePlan<T % kPeriod, T, (T + 1 < kQ16 ? T + 1 : T), (T > 0 ? T - 1 : 0), T, (T + 1 < kQ16 ? T + 1 : kNoMask), (T + 2 < kQ16),
                               (T + 1 < kQ16)>;
 
-template <int D, typename TO, bool CAUSAL>
-__device__ __forceinline__ bool packed_item(const packed::Params& p, const packed::Item& item, char* smem_raw);
+// A part of an item: the tiles [first, behind) of its keys.  SPLIT kernels cut items with many tiles where there are too few
+// of them to fill the chip: every part leaves its sums, and the last one to do so adds them up.
+constexpr int kMostParts = 4, kPartTiles = 8;  // parts of an item at most, tiles of a part at least
+struct Part {
+  int parts, first, behind;
+};
+template <int D, typename TO, bool CAUSAL, bool SPLIT>
+__device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Item item, const Part& part, char* smem_raw);
 
-template <int D, typename TO, bool CAUSAL>
+template <int D, typename TO, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(kThreads, kQ16 == 2 ? 2 : 1) void attn_fwd_kernel_packed(const packed::Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   bool again;
   {
-    const packed::Item item = packed::find_item(p, kPackedRows, CAUSAL, (int)(threadIdx.x & 63));
+    Part part{1, 0, 0};
+    const uint32_t nth = SPLIT ? blockIdx.x / p.items : 0;  // number of the part
+    const packed::Item item = packed::find_item(p, SPLIT ? blockIdx.x - nth * p.items : blockIdx.x, kPackedRows, CAUSAL, (int)(threadIdx.x & 63));
     if (!item.it.there) return;
     // rows that see no key: at most the first ones of a sequence with more queries than keys
     again = item.it.nk == 0 || item.a0 < 0;
-    if (!again) again = packed_item<D, TO, CAUSAL>(p, item, smem_raw);
+    if (!again) {
+      part.behind = CAUSAL ? item.a0 / kBc + kQ16 : (item.it.nk - 1) / kBc + 1;  // tiles of the item
+      if constexpr (SPLIT) {
+        const int tiles = part.behind, wanted = tiles / kPartTiles;
+        part.parts = wanted < 1 ? 1 : (wanted < p.parts ? wanted : p.parts);
+        if ((int)nth >= part.parts) return;
+        part.first = (int)nth * tiles / part.parts;
+        part.behind = ((int)nth + 1) * tiles / part.parts;
+      }
+      again = packed_item<D, TO, CAUSAL, SPLIT>(p, item, part, smem_raw);
+    } else if (nth > 0) {
+      return;
+    }
   }
   if (again) {
     // (rare: the arguments are read again here, rather than kept in registers all the while)
@@ -50,7 +70,7 @@ __global__ __launch_bounds__(kThreads, kQ16 == 2 ? 2 : 1) void attn_fwd_kernel_p
     asm volatile("" : "+s"(late));
     int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     asm volatile("" : "+v"(lane));
-    const packed::Item item = packed::find_item(*late, kPackedRows, CAUSAL, lane);
+    const packed::Item item = packed::find_item(*late, SPLIT ? blockIdx.x % late->items : blockIdx.x, kPackedRows, CAUSAL, lane);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 #pragma unroll 1
     for (int q = 0; q < kQ16; ++q) {
@@ -61,9 +81,10 @@ __global__ __launch_bounds__(kThreads, kQ16 == 2 ? 2 : 1) void attn_fwd_kernel_p
 #endif
 }
 
-// The item on the pipelined body.  True: this wave's rows hold NaN or infinities and so do the values of its diagonal.
-template <int D, typename TO, bool CAUSAL>
-__device__ __forceinline__ bool packed_item(const packed::Params& p, const packed::Item& item, char* smem_raw) {
+// The item, or a part of it, on the pipelined body.  True: this wave's rows hold NaN or infinities and so do the values of
+// its diagonal.
+template <int D, typename TO, bool CAUSAL, bool SPLIT>
+__device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Item item, const Part& part, char* smem_raw) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = Cfg<D>;
   constexpr int EK = kElemKindOf<TO>;
@@ -76,11 +97,18 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, const packe
   const int n16 = lane & 15;
   const int g = lane >> 4;
   const int d = p.d;
+  if constexpr (SPLIT) {
+    // the keys in front of the part are not there for anything below
+    item.it.k0 += part.first * kBc;
+    item.it.nk -= part.first * kBc;
+    item.a0 -= part.first * kBc;
+  }
   const packed::Tile& it = item.it;
   const int32_t head = item.head, kvh = item.kvh, row0 = item.row0, a0 = item.a0;
+  const int32_t seen = CAUSAL ? a0 - row0 : 0;  // keys that a row sees, less its number and one
   // Tiles in front of the end: the diagonal's kQ16 (rows that do not exist make some of them idle), or the last one,
   // which may be partly there
-  const int full = CAUSAL ? a0 / kBc : (it.nk - 1) / kBc;
+  const int full = SPLIT ? part.behind - part.first - (CAUSAL ? kQ16 : 1) : (CAUSAL ? a0 / kBc : (it.nk - 1) / kBc);
   const int lead = (kPeriod - full % kPeriod) % kPeriod;
   const ScaleSplit sc{p.scale_log2, kDeferLog2 / p.scale_log2};
 
@@ -179,7 +207,7 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, const packe
     }
   }
   const LaneAddr<D> la = make_lane_addr<D>(lane, k_ring, v_ring);
-  const QueryLimit limit_causal{row_n + it.nk - it.nq + 1};
+  const QueryLimit limit_causal{row_n + seen + 1};
   const auto limit = [&]() __attribute__((always_inline)) {
     if constexpr (CAUSAL) return limit_causal; else return (int)it.nk;
   }();
@@ -297,8 +325,14 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, const packe
       if (++t == full) break;
     }
   }
-  constexpr int kLastQ = CAUSAL ? kQ16 - 1 : 0;  // first query block that sees the last tile
-  if constexpr (CAUSAL) {
+  // The end's tiles.  (Of a part that is not the last one these are like the others, so that all query blocks run through
+  // all of them, with masks that leave such a part's scores as they are: a second end beside the diagonal's made the
+  // compiler spill 216 registers.)
+  if constexpr (SPLIT && CAUSAL) {
+    static_assert(kQ16 == 2, "two tiles");
+    tile_iter(TilePlan<0, 0, 0, 0, 0, kMaskAll, false, true>{}, full);
+    tile_iter(TilePlan<1, 0, 0, 0, kMaskAll, kNoMask, false, false>{}, full + 1);
+  } else if constexpr (CAUSAL) {
     tile_iter(DiagonalPlan<0>{}, full);
     tile_iter(DiagonalPlan<1>{}, full + 1);
     if constexpr (kQ16 == 4) {
@@ -308,18 +342,18 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, const packe
   } else {
     tile_iter(TilePlan<0, 0, 0, 0, kMaskAll, kNoMask, false, false>{}, full);
   }
-  // PV of the last block
-  {
-    drain_o(o);
+
+  // ---- the second product of the last block -----------------------------------------------------------------------
+  constexpr int kLastQ = CAUSAL && !SPLIT ? kQ16 - 1 : 0, kLastSlot = ((CAUSAL ? 2 * kQ16 : 2) - 1) % kVBlocks;
+  drain_o(o);
 #pragma unroll
-    for (int b = 0; b < kDv16; ++b) {
-      const f16x8 vf = read_v<D>((uint32_t)((CAUSAL ? 2 * kQ16 - 1 : 1) % kVBlocks * kBlkBytes), la, b);
+  for (int b = 0; b < kDv16; ++b) {
+    const f16x8 vf = read_v<D>((uint32_t)(kLastSlot * kBlkBytes), la, b);
 #pragma unroll
-      for (int q = kLastQ; q < kQ16; ++q) mfma_o<true, EK>(o[q][b], vf, pB[q]);
-    }
-    drain_o(o);
-    drain_lsum<D>(lsum);
+    for (int q = kLastQ; q < kQ16; ++q) mfma_o<true, EK>(o[q][b], vf, pB[q]);
   }
+  drain_o(o);
+  drain_lsum<D>(lsum);
 
   // ---- epilogue ----------------------------------------------------------------------------------------------
   // (the lane's number again, from the hardware: nothing of it is kept through the iterations)
@@ -327,26 +361,110 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, const packe
   asm volatile("" : "+v"(lane_e));
   const int n_e = lane_e & 15, g_e = lane_e >> 4;
   bool odd = false;
-#pragma unroll
-  for (int q = 0; q < kQ16; ++q) {
-    const float inv = __builtin_amdgcn_rcpf(quad_lane_sum(lsum[q][0], lane_e));
+  // two neighbouring tiles of O^T of query block q, as 8 consecutive columns of one of them per lane
+  auto store_pair = [&](int q, int b, const f32x4& x, const f32x4& y, float inv) __attribute__((always_inline)) {
     const bool there = (uint32_t)(row0 + 16 * wave + n_e + 64 * q) < (uint32_t)it.nq;
+    const f32x4 xs = x * inv, ys = y * inv;
+    const u32x2 xu = {pack2<EK>(xs[0], xs[1]), pack2<EK>(xs[2], xs[3])};
+    const u32x2 yu = {pack2<EK>(ys[0], ys[1]), pack2<EK>(ys[2], ys[3])};
+    u32x4 out;
 #pragma unroll
-    for (int b = 0; b < kDv16; b += 2) {
-      const f32x4 xs = o[q][b] * inv, ys = o[q][b + 1] * inv;
-      const u32x2 xu = {pack2<EK>(xs[0], xs[1]), pack2<EK>(xs[2], xs[3])};
-      const u32x2 yu = {pack2<EK>(ys[0], ys[1]), pack2<EK>(ys[2], ys[3])};
-      u32x4 out;
+    for (int w = 0; w < 2; ++w) {
+      auto r = __builtin_amdgcn_permlane16_swap(xu[w], yu[w], false, false);
+      out[w] = r[0];
+      out[2 + w] = r[1];
+    }
+    const int dv = 16 * (b + (g_e & 1)) + 8 * (g_e >> 1);
+    const uint32_t off = (there && dv < d) ? (uint32_t)(64 * q + 16 * wave + n_e) * o_row + (uint32_t)dv * 2u : kOob;
+    __builtin_amdgcn_raw_buffer_store_b128(out, o_rs, off, 0, 0);
+    if constexpr (CAUSAL) odd |= there && packed::holds_not_finite<EK == kBF16>(out);
+  };
+  if (!SPLIT || part.parts == 1) {
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        auto r = __builtin_amdgcn_permlane16_swap(xu[w], yu[w], false, false);
-        out[w] = r[0];
-        out[2 + w] = r[1];
+    for (int q = 0; q < kQ16; ++q) {
+      const float inv = __builtin_amdgcn_rcpf(quad_lane_sum(lsum[q][0], lane_e));
+#pragma unroll
+      for (int b = 0; b < kDv16; b += 2) store_pair(q, b, o[q][b], o[q][b + 1], inv);
+    }
+  } else if constexpr (SPLIT) {
+    // Parts go to memory and come from there past the L2s (sc0 sc1), which the XCDs do not share; the last one to take a
+    // ticket adds them up in their order.
+    constexpr int kThrough = 17;
+    constexpr uint32_t kPartFloats = (uint32_t)(kPackedRows * D);
+    // (the arguments are read again here, rather than kept in registers through the iterations)
+    const packed::Params* late = (const packed::Params*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(late));
+    const uint32_t nth = blockIdx.x / late->items, number = blockIdx.x - nth * late->items;
+    const uint32_t slots = late->items * (uint32_t)late->parts;
+    const __amdgpu_buffer_rsrc_t part_o = __builtin_amdgcn_make_buffer_rsrc(late->part_o, 0, (int)(slots * kPartFloats * 4u), 0x00020000);
+    const __amdgpu_buffer_rsrc_t part_ml = __builtin_amdgcn_make_buffer_rsrc(late->part_ml, 0, (int)(slots * (uint32_t)kPackedRows * 8u), 0x00020000);
+    const uint32_t slot0 = number * (uint32_t)late->parts;
+    auto o_at = [&](uint32_t slot, int q, int b) __attribute__((always_inline)) {
+      return (slot * kPartFloats + (uint32_t)((((wave * kQ16 + q) * kDv16 + b) * 64 + lane_e) * 4)) * 4u;
+    };
+    auto ml_at = [&](uint32_t slot, int q) __attribute__((always_inline)) {
+      return (slot * (uint32_t)kPackedRows + (uint32_t)(64 * q + 16 * wave + n_e)) * 8u;
+    };
+#pragma unroll
+    for (int q = 0; q < kQ16; ++q) {
+      const float l = quad_lane_sum(lsum[q][0], lane_e);
+#pragma unroll
+      for (int b = 0; b < kDv16; ++b) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[q][b]), part_o, o_at(slot0 + nth, q, b), 0, kThrough);
       }
-      const int dv = 16 * (b + (g_e & 1)) + 8 * (g_e >> 1);
-      const uint32_t off = (there && dv < d) ? (uint32_t)(64 * q + 16 * wave + n_e) * o_row + (uint32_t)dv * 2u : kOob;
-      __builtin_amdgcn_raw_buffer_store_b128(out, o_rs, off, 0, 0);
-      if constexpr (CAUSAL) odd |= there && packed::holds_not_finite<EK == kBF16>(out);
+      if (g_e == 0) {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(st[q].mc * sc.c), __float_as_uint(l)}, part_ml,
+                                              ml_at(slot0 + nth, q), 0, kThrough);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t* const said = (uint32_t*)smem_raw;  // (the rings are done with)
+    if (tid == 0) *said = __hip_atomic_fetch_add(late->tickets + number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*said != (uint32_t)part.parts - 1) return false;
+    asm volatile("" ::: "memory");
+    if (tid == 0) __hip_atomic_store(late->tickets + number, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll 1
+    for (int q = 0; q < kQ16; ++q) {
+      float w[kMostParts], l = 0.f, m = -INFINITY;
+      u32x2 ml[kMostParts];
+#pragma unroll
+      for (int i = 0; i < kMostParts; ++i) {
+        ml[i] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, ml_at(slot0 + (uint32_t)(i < part.parts ? i : part.parts - 1), q), 0, kThrough);
+      }
+#pragma unroll
+      for (int i = 0; i < kMostParts; ++i) m = fmaxf(m, __uint_as_float(ml[i][0]));
+#pragma unroll
+      for (int i = 0; i < kMostParts; ++i) {
+        w[i] = i < part.parts ? fast_exp2(__uint_as_float(ml[i][0]) - m) : 0.f;
+        l += i < part.parts ? w[i] * __uint_as_float(ml[i][1]) : 0.f;
+      }
+      const float inv = __builtin_amdgcn_rcpf(l);
+      constexpr int kTogether = 4;  // tiles of O^T whose parts are fetched together
+#pragma unroll
+      for (int b0 = 0; b0 < kDv16; b0 += kTogether) {
+        f32x4 x[kTogether][kMostParts];
+#pragma unroll
+        for (int b = 0; b < kTogether; ++b) {
+#pragma unroll
+          for (int i = 0; i < kMostParts; ++i) {
+            x[b][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    part_o, o_at(slot0 + (uint32_t)(i < part.parts ? i : part.parts - 1), q, b0 + b), 0, kThrough));
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kTogether; ++b) {
+          f32x4 sum = x[b][0] * w[0];
+#pragma unroll
+          for (int i = 1; i < kMostParts; ++i) {
+            if (i < part.parts) sum += x[b][i] * w[i];
+          }
+          x[b][0] = sum;
+        }
+#pragma unroll
+        for (int b = 0; b < kTogether; b += 2) store_pair(q, b0 + b, x[b][0], x[b + 1][0], inv);
+      }
     }
   }
   if constexpr (CAUSAL) {

@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
-#include <cstdlib>
 
 #include "attn_packed_mfma.hpp"
 #include "host.hpp"
@@ -29,7 +28,7 @@ int launch(const packed::Params& p, hipStream_t stream) {
     if (e != hipSuccess) return set_error(FLASH_HIP_ERR_LDS, "Failed to set dynamic shared memory size %u: %s", kLds, hipGetErrorString(e));
     if (cached) done.fetch_or((uint64_t)1 << dev, std::memory_order_release);
   }
-  hipLaunchKernelGGL(KERNEL, dim3((uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads)), dim3(m16::kThreads), kLds, stream, p);
+  hipLaunchKernelGGL(KERNEL, dim3(p.items * (uint32_t)p.parts), dim3(m16::kThreads), kLds, stream, p);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FLASH_HIP_ERR_RUNTIME, "flash_fwd_packed: kernel launch failed: %s", hipGetErrorString(e));
   return FLASH_HIP_OK;
@@ -44,25 +43,57 @@ struct HalfOut<m16::bf16_out> {
   using type = m16h::bf16_out;
 };
 
-template <int D, typename TO>
-int launch(packed::Params p, hipStream_t stream) {
-  // Long sequences with work for every compute unit take the 256-row items: each K/V tile is fetched and read from LDS by
-  // half as many waves.  Shorter ones take the 128-row items, two workgroups to a compute unit, of which one computes
-  // while the other starts or ends.  Measured, 128-row / 256-row, us: 32 heads of 128 over 8, 16 x 512 rows 67 / 74,
-  // 8 x 1024 88 / 97, 4 x 2048 139 / 141, 2 x 4096 243 / 239, 8192 457 / 442, 16384 1775 / 1719; 32 heads of 64,
-  // 8 x 1024 56 / 66, 2 x 4096 152 / 154, 8192 288 / 282; 160 items of 128 rows (16 heads of 64) 45 / 67.
-  static const char* force = getenv("PK_HALF");
-  const bool half = force ? force[0] == '1' : (int64_t)p.total_k < (int64_t)4096 * p.sequences || (int64_t)p.total_q / m16::kPackedRows * p.heads < 512;
-  // a sequence has at most two tiles more than whole ones among its rows (its first one may be short, and its last one)
-  const int64_t rows = half ? m16h::kPackedRows : m16::kPackedRows;
+// Long sequences with work for every compute unit take the 256-row items: each K/V tile is fetched and read from LDS by half
+// as many waves.  Shorter ones take the 128-row items, two workgroups to a compute unit, of which one computes while
+// the other starts or ends.  Measured, 128-row / 256-row, us: 32 heads of 128 over 8, 16 x 512 rows 67 / 74, 8 x 1024
+// 88 / 97, 4 x 2048 139 / 141, 2 x 4096 243 / 239, 8192 457 / 442, 16384 1775 / 1719; 32 heads of 64, 8 x 1024 56 / 66,
+// 2 x 4096 152 / 154, 8192 288 / 282; 160 items of 128 rows (16 heads of 64) 45 / 67.
+bool take_half(const packed::Params& p) {
+  return (int64_t)p.total_k < (int64_t)4096 * p.sequences || (int64_t)p.total_q / m16::kPackedRows * p.heads < 512;
+}
+// The grid's tiles: a sequence has at most two more than whole ones among its rows (its first one may be short, and its
+// last one).
+void set_grid(packed::Params& p, int64_t rows) {
   p.tiles = (uint32_t)(p.total_q / rows + 2 * p.sequences);
+  p.items = (uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads);
+  p.parts = 1;
+}
+// Fewer 128-row items than three quarters of the places on the chip (two for each of 256 compute units), with enough keys to
+// cut: the keys of an item are dealt to several workgroups.  Twice the places are aimed at, since the items are not alike and
+// the grid holds some that do not exist.
+int parts_of(const packed::Params& p) {
+  constexpr int64_t kPlaces = 512;
+  if (!take_half(p) || p.total_k < 2 * m16h::kPartTiles * kBc) return 1;
+  packed::Params h = p;
+  set_grid(h, m16h::kPackedRows);
+  static_assert(kPlaces * 3 / 4 * 4 <= FLASH_PACKED_TICKET_BYTES, "one ticket for each item that is cut");
+  if ((int64_t)h.items * 4 >= kPlaces * 3) return 1;
+  const int64_t wanted = 2 * kPlaces / h.items;
+  return (int)(wanted < m16h::kMostParts ? wanted : m16h::kMostParts);
+}
+// floats of a part of an item: its rows of O^T, and their reference and sum
+int64_t part_floats(const packed::Params& p) { return (int64_t)m16h::kPackedRows * ((p.d <= 64 ? 64 : 128) + 2); }
+
+template <int D, typename TO>
+int launch(packed::Params p, void* workspace, hipStream_t stream) {
   using TH = typename HalfOut<TO>::type;
-  if (half) {
-    return p.causal ? launch<m16h::attn_fwd_kernel_packed<D, TH, true>, m16h::kPackedLds<D>>(p, stream)
-                    : launch<m16h::attn_fwd_kernel_packed<D, TH, false>, m16h::kPackedLds<D>>(p, stream);
+  if (take_half(p)) {
+    const int parts = workspace ? parts_of(p) : 1;
+    set_grid(p, m16h::kPackedRows);
+    if (parts > 1) {
+      p.parts = parts;
+      p.tickets = (uint32_t*)workspace;
+      p.part_o = (float*)((char*)workspace + FLASH_PACKED_TICKET_BYTES);
+      p.part_ml = p.part_o + (int64_t)p.items * parts * m16h::kPackedRows * D;
+      return p.causal ? launch<m16h::attn_fwd_kernel_packed<D, TH, true, true>, m16h::kPackedLds<D>>(p, stream)
+                      : launch<m16h::attn_fwd_kernel_packed<D, TH, false, true>, m16h::kPackedLds<D>>(p, stream);
+    }
+    return p.causal ? launch<m16h::attn_fwd_kernel_packed<D, TH, true, false>, m16h::kPackedLds<D>>(p, stream)
+                    : launch<m16h::attn_fwd_kernel_packed<D, TH, false, false>, m16h::kPackedLds<D>>(p, stream);
   }
-  return p.causal ? launch<m16::attn_fwd_kernel_packed<D, TO, true>, m16::kPackedLds<D>>(p, stream)
-                  : launch<m16::attn_fwd_kernel_packed<D, TO, false>, m16::kPackedLds<D>>(p, stream);
+  set_grid(p, m16::kPackedRows);
+  return p.causal ? launch<m16::attn_fwd_kernel_packed<D, TO, true, false>, m16::kPackedLds<D>>(p, stream)
+                  : launch<m16::attn_fwd_kernel_packed<D, TO, false, false>, m16::kPackedLds<D>>(p, stream);
 }
 
 }  // namespace
@@ -74,9 +105,17 @@ bool packed_mfma_takes(const packed::Params& p) {
          packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads) < (1ull << 31);
 }
 
-int launch_packed_mfma(packed::Params p, bool bf16, hipStream_t stream) {
-  if (p.d <= 64) return bf16 ? launch<64, m16::bf16_out>(p, stream) : launch<64, f16>(p, stream);
-  return bf16 ? launch<128, m16::bf16_out>(p, stream) : launch<128, f16>(p, stream);
+int64_t packed_mfma_workspace(const packed::Params& p) {
+  const int parts = packed_mfma_takes(p) ? parts_of(p) : 1;
+  if (parts == 1) return 0;
+  packed::Params h = p;
+  set_grid(h, m16h::kPackedRows);
+  return FLASH_PACKED_TICKET_BYTES + (int64_t)h.items * parts * part_floats(p) * 4;
+}
+
+int launch_packed_mfma(const packed::Params& p, bool bf16, void* workspace, hipStream_t stream) {
+  if (p.d <= 64) return bf16 ? launch<64, m16::bf16_out>(p, workspace, stream) : launch<64, f16>(p, workspace, stream);
+  return bf16 ? launch<128, m16::bf16_out>(p, workspace, stream) : launch<128, f16>(p, workspace, stream);
 }
 
 }  // namespace flash_hip

@@ -166,6 +166,49 @@ int launch_packed_direct(flash_hip::packed::Params p, hipStream_t stream) {
   return launched("flash_fwd_packed");
 }
 
+// The kernel's arguments, for what flash_fwd_packed takes.  Without `memory` the sizes and strides alone are looked at.
+int plan_packed(const flash_packed_args* a, bool memory, flash_hip::packed::Params* out) {
+  REFUSE_IF(!a, "null flash_packed_args");
+  CHECK(check_16bit(a->dtype));
+  CHECK(check_heads(a->q_heads, a->kv_heads, a->d));
+  CHECK(check_scale(a->softmax_scale));
+  REFUSE_IF(a->causal != 0 && a->causal != 1, "causal must be 0 or 1 (got %d)", a->causal);
+  REFUSE_IF(a->sequences < 0 || a->sequences > kMostIndex || a->total_q < 0 || a->total_q > kMostIndex || a->total_k < 0 || a->total_k > kMostIndex,
+            "sequences and rows must be between 0 and 2^30 (got %lld sequences, %lld queries, %lld keys)", (long long)a->sequences,
+            (long long)a->total_q, (long long)a->total_k);
+  if (a->sequences == 0 || a->total_q == 0) return FLASH_HIP_OK;
+  REFUSE_IF(memory && (!a->q || !a->o || ((!a->k || !a->v) && a->total_k > 0)), "null tensor pointer");
+  REFUSE_IF(memory && (!a->cu_seqlens_q || !a->cu_seqlens_k), "null cu_seqlens");
+  CHECK(check_rows("q", memory ? a->q : nullptr, a->q_token_stride, a->total_q, a->q_head_stride, a->q_heads, 2, 16));
+  CHECK(check_rows("k", memory ? a->k : nullptr, a->k_token_stride, a->total_k, a->k_head_stride, a->kv_heads, 2, 16));
+  CHECK(check_rows("v", memory ? a->v : nullptr, a->v_token_stride, a->total_k, a->v_head_stride, a->kv_heads, 2, 16));
+  CHECK(check_rows("out", memory ? a->o : nullptr, a->o_token_stride, a->total_q, a->o_head_stride, a->q_heads, 2, 16));
+  flash_hip::packed::Params& p = *out;
+  p.q = (const char*)a->q;
+  p.k = (const char*)a->k;
+  p.v = (const char*)a->v;
+  p.o = (char*)a->o;
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_k = a->cu_seqlens_k;
+  p.q_token = a->q_token_stride * 2;
+  p.q_head = a->q_head_stride * 2;
+  p.k_token = a->k_token_stride * 2;
+  p.k_head = a->k_head_stride * 2;
+  p.v_token = a->v_token_stride * 2;
+  p.v_head = a->v_head_stride * 2;
+  p.o_token = a->o_token_stride * 2;
+  p.o_head = a->o_head_stride * 2;
+  p.sequences = (int32_t)a->sequences;
+  p.total_q = (int32_t)a->total_q;
+  p.total_k = (int32_t)a->total_k;
+  p.heads = (int32_t)a->q_heads;
+  p.kv_heads = (int32_t)a->kv_heads;
+  p.d = (int32_t)a->d;
+  p.causal = a->causal;
+  p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  return FLASH_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -264,47 +307,22 @@ int flash_cache_append(const flash_append_args* a, const flash_paged_cache* c, v
   return launched("flash_cache_append");
 }
 
-int flash_fwd_packed(const flash_packed_args* a, void* hip_stream) {
-  REFUSE_IF(!a, "null flash_packed_args");
-  CHECK(check_16bit(a->dtype));
-  CHECK(check_heads(a->q_heads, a->kv_heads, a->d));
-  CHECK(check_scale(a->softmax_scale));
-  REFUSE_IF(a->causal != 0 && a->causal != 1, "causal must be 0 or 1 (got %d)", a->causal);
-  REFUSE_IF(a->sequences < 0 || a->sequences > kMostIndex || a->total_q < 0 || a->total_q > kMostIndex || a->total_k < 0 || a->total_k > kMostIndex,
-            "sequences and rows must be between 0 and 2^30 (got %lld sequences, %lld queries, %lld keys)", (long long)a->sequences,
-            (long long)a->total_q, (long long)a->total_k);
-  if (a->sequences == 0 || a->total_q == 0) return FLASH_HIP_OK;
-  REFUSE_IF(!a->q || !a->o || ((!a->k || !a->v) && a->total_k > 0), "null tensor pointer");
-  REFUSE_IF(!a->cu_seqlens_q || !a->cu_seqlens_k, "null cu_seqlens");
-  CHECK(check_rows("q", a->q, a->q_token_stride, a->total_q, a->q_head_stride, a->q_heads, 2, 16));
-  CHECK(check_rows("k", a->k, a->k_token_stride, a->total_k, a->k_head_stride, a->kv_heads, 2, 16));
-  CHECK(check_rows("v", a->v, a->v_token_stride, a->total_k, a->v_head_stride, a->kv_heads, 2, 16));
-  CHECK(check_rows("out", a->o, a->o_token_stride, a->total_q, a->o_head_stride, a->q_heads, 2, 16));
+int64_t flash_fwd_packed_workspace_bytes(const flash_packed_args* args) {
   flash_hip::packed::Params p{};
-  p.q = (const char*)a->q;
-  p.k = (const char*)a->k;
-  p.v = (const char*)a->v;
-  p.o = (char*)a->o;
-  p.cu_q = a->cu_seqlens_q;
-  p.cu_k = a->cu_seqlens_k;
-  p.q_token = a->q_token_stride * 2;
-  p.q_head = a->q_head_stride * 2;
-  p.k_token = a->k_token_stride * 2;
-  p.k_head = a->k_head_stride * 2;
-  p.v_token = a->v_token_stride * 2;
-  p.v_head = a->v_head_stride * 2;
-  p.o_token = a->o_token_stride * 2;
-  p.o_head = a->o_head_stride * 2;
-  p.sequences = (int32_t)a->sequences;
-  p.total_q = (int32_t)a->total_q;
-  p.total_k = (int32_t)a->total_k;
-  p.heads = (int32_t)a->q_heads;
-  p.kv_heads = (int32_t)a->kv_heads;
-  p.d = (int32_t)a->d;
-  p.causal = a->causal;
-  p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  if (plan_packed(args, false, &p) != FLASH_HIP_OK) return -1;
+  return p.total_q > 0 ? flash_hip::packed_mfma_workspace(p) : 0;
+}
+int flash_fwd_packed(const flash_packed_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+  flash_hip::packed::Params p{};
+  CHECK(plan_packed(a, true, &p));
+  if (p.total_q == 0) return FLASH_HIP_OK;
+  if (workspace) {
+    const int64_t need = flash_hip::packed_mfma_workspace(p);
+    REFUSE_IF(workspace_bytes < need, "workspace of %lld bytes is too small: %lld needed", (long long)workspace_bytes, (long long)need);
+    REFUSE_IF((uintptr_t)workspace % 16 != 0, "workspace must be 16-byte aligned");
+  }
   const hipStream_t stream = (hipStream_t)hip_stream;
-  if (flash_hip::packed_mfma_takes(p)) return flash_hip::launch_packed_mfma(p, a->dtype == FLASH_BF16, stream);
+  if (flash_hip::packed_mfma_takes(p)) return flash_hip::launch_packed_mfma(p, a->dtype == FLASH_BF16, workspace, stream);
   using namespace flash_hip::direct;
   if (a->d <= 64) return a->dtype == FLASH_F16 ? launch_packed_direct<64, kHalf>(p, stream) : launch_packed_direct<64, kBfloat>(p, stream);
   return a->dtype == FLASH_F16 ? launch_packed_direct<128, kHalf>(p, stream) : launch_packed_direct<128, kBfloat>(p, stream);

@@ -71,11 +71,12 @@ void wait_for(const c10::hip::HIPStreamMasqueradingAsCUDA& stream) {
   if (e != hipSuccess) throw std::runtime_error(hipGetErrorString(e));
 }
 
-// Zero-filled scratch for flash_decode_paged.  Work on one stream runs in order, so its calls share a buffer that is
-// filled once, on their first call (and again when a larger one is needed).  A graph under capture gets one of its own,
-// filled by a node of the graph: it may be replayed on any stream, beside any other.  So does a call on a stream that torch
-// did not make, whose handle may come to stand for another stream.
-Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradingAsCUDA& stream, int64_t need) {
+// Scratch whose bytes [zeros.first, zeros.second) (-1: up to its end) are zero, and left zero by the calls that use it; one
+// kind of scratch has one value of zeros.first.  Work on one stream runs in order, so its calls share a buffer that is filled
+// once, on their first call (and again when a larger one is needed).  A graph under capture gets one of its own, filled by a
+// node of the graph: it may be replayed on any stream, beside any other.  So does a call on a stream that torch did not
+// make, whose handle may come to stand for another stream.
+Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradingAsCUDA& stream, int64_t need, std::pair<int64_t, int64_t> zeros) {
   const auto options = at::TensorOptions().dtype(at::kByte).device(device);
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess) throw std::runtime_error("hipStreamIsCapturing failed");
@@ -83,14 +84,15 @@ Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradin
   const bool own_stream = id == 0 || (id & 1) != 0;  // torch's numbering: the default stream, and the streams of its pools
   auto fresh = [&](int64_t bytes) {
     Tensor t = at::empty({bytes}, options);
-    t.narrow(0, FLASH_DECODE_PARTS_BYTES, bytes - FLASH_DECODE_PARTS_BYTES).zero_();
+    t.slice(0, zeros.first, zeros.second < 0 ? bytes : zeros.second).zero_();
     return t;
   };
   if (capture != hipStreamCaptureStatusNone || !own_stream) return fresh(need);
   static std::mutex mutex;
-  static auto& buffers = *new std::map<std::pair<int, c10::StreamId>, Tensor>;  // (never destroyed: the allocator may be gone by then)
+  // (never destroyed: the allocator may be gone by then)
+  static auto& buffers = *new std::map<std::tuple<int, c10::StreamId, int64_t>, Tensor>;
   const std::lock_guard<std::mutex> lock(mutex);
-  Tensor& t = buffers[{device.index(), id}];
+  Tensor& t = buffers[{device.index(), id, zeros.first}];
   if (!t.defined() || t.numel() < need) t = fresh(need + (1 << 16));
   return t;
 }
@@ -174,7 +176,6 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
             cu_q.size(0), " and ", cu_k.size(0));
   refuse_if(!cu_k_given && k.size(0) != q.size(0), "without cu_seqlens_k there must be as many keys as queries, got ", k.size(0), " and ", q.size(0));
   check_no_grad({&q, &k, &v});
-  if (out_given) refuse_if(out_given->sizes() != q.sizes() || out_given->scalar_type() != q.scalar_type(), "out must have the shape and type of q");
   a.sequences = cu_q.size(0) - 1;
   a.total_q = q.size(0);
   a.total_k = k.size(0);
@@ -183,10 +184,22 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   a.d = q.size(2);
   a.causal = causal ? 1 : 0;
   a.softmax_scale = scale_of(softmax_scale, a.d);
+  a.q_token_stride = q.stride(0);
+  a.q_head_stride = q.stride(1);
+  a.k_token_stride = k.stride(0);
+  a.k_head_stride = k.stride(1);
+  a.v_token_stride = v.stride(0);
+  a.v_head_stride = v.stride(1);
+  a.o_token_stride = a.q_heads * a.d;
+  a.o_head_stride = a.d;
+  if (out_given) {
+    output_for(q, out_given);
+    a.o_token_stride = out_given->stride(0);
+    a.o_head_stride = out_given->stride(1);
+  }
   // what needs no memory is refused before the device is looked at
-  flash_packed_args sizes = a;
-  sizes.total_q = 0;
-  raise(flash_fwd_packed(&sizes, nullptr));
+  const int64_t need = flash_fwd_packed_workspace_bytes(&a);
+  if (need < 0) throw std::invalid_argument(flash_hip_last_error());
   check_device(q, {&k, &v, &cu_q, &cu_k, &or_none(out_given)});
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   Tensor o = output_for(q, out_given);
@@ -196,16 +209,10 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   a.o = o.data_ptr();
   a.cu_seqlens_q = static_cast<const int32_t*>(cu_q.const_data_ptr());
   a.cu_seqlens_k = static_cast<const int32_t*>(cu_k.const_data_ptr());
-  a.q_token_stride = q.stride(0);
-  a.q_head_stride = q.stride(1);
-  a.k_token_stride = k.stride(0);
-  a.k_head_stride = k.stride(1);
-  a.v_token_stride = v.stride(0);
-  a.v_head_stride = v.stride(1);
-  a.o_token_stride = o.stride(0);
-  a.o_head_stride = o.stride(1);
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
-  raise(flash_fwd_packed(&a, stream.stream()));
+  Tensor scratch;
+  if (need > 0) scratch = stream_workspace(q.device(), stream, need, {0, FLASH_PACKED_TICKET_BYTES});
+  raise(flash_fwd_packed(&a, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
   if (sync) wait_for(stream);
   return o;
 }
@@ -248,7 +255,7 @@ std::tuple<Tensor, Tensor> decode_paged(const Tensor& q, const Tensor& k_cache, 
     a.lse = static_cast<float*>(lse.data_ptr());
   }
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
-  if (need > 0) scratch = workspace ? *workspace : stream_workspace(q.device(), stream, need);
+  if (need > 0) scratch = workspace ? *workspace : stream_workspace(q.device(), stream, need, {FLASH_DECODE_PARTS_BYTES, -1});
   raise(flash_decode_paged(&a, &c, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
   if (sync) wait_for(stream);
   return {o, lse};

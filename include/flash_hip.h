@@ -264,7 +264,17 @@ typedef struct flash_packed_args {
   int32_t causal;                /* 0 or 1 */
   int32_t dtype;                 /* FLASH_F16 or FLASH_BF16 */
 } flash_packed_args;
-int flash_fwd_packed(const flash_packed_args* args, void* hip_stream);
+/*
+ * `workspace` (may be NULL): device memory, 16-byte aligned, flash_fwd_packed_workspace_bytes(...) bytes.  With it, calls
+ * whose rows are too few for the whole chip deal the keys of a row to several workgroups; without it they take longer.
+ * Its first FLASH_PACKED_TICKET_BYTES bytes are zero before its first use, and every call leaves them zero, so it serves
+ * any number of calls, of any shape, one after the other; it is not shared by calls that may overlap in time.
+ */
+#define FLASH_PACKED_TICKET_BYTES 2048ll
+int flash_fwd_packed(const flash_packed_args* args, void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* 0 for a call that would not use one, -1 (and an error text) for what flash_fwd_packed refuses.  Looks at sizes and strides
+ * only; does not touch the GPU. */
+int64_t flash_fwd_packed_workspace_bytes(const flash_packed_args* args);
 
 /*
  * A paged cache: position j of sequence b lies in page page_table[b][j / page_size], slot j % page_size.
@@ -287,10 +297,10 @@ typedef struct flash_paged_cache {
  * Attention of one new token of every sequence over the cache: q [sequences, q_heads, d] (16-bit, dtype), whose key
  * and value are in the cache already.  lse (may be NULL): [sequences, q_heads], contiguous, the natural logarithm of
  * the sum of the weights exp(softmax_scale q.k).  A sequence of length 0 gets zeros and -inf.
- * `workspace`: device memory, 16-byte aligned, flash_decode_paged_workspace_bytes(...) bytes, filled with zeros before its
- * first use (what lies behind its first FLASH_DECODE_PARTS_BYTES; the rest may hold anything).  Every call leaves the part of it that has to be zero as it found it, so it serves any number of calls, of any
- * shape, one after the other; it is not to be touched until a call's work has finished, nor shared by calls that may
- * overlap in time (two captured graphs among them).
+ * `workspace`: device memory, 16-byte aligned, flash_decode_paged_workspace_bytes(...) bytes.  What lies behind its first
+ * FLASH_DECODE_PARTS_BYTES is zero before its first use (the rest may hold anything), and every call leaves that zero, so it
+ * serves any number of calls, of any shape, one after the other; it is not to be touched until a call's work has finished,
+ * nor shared by calls that may overlap in time (two captured graphs among them).
  */
 typedef struct flash_decode_args {
   const void* q;

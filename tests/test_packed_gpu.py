@@ -222,3 +222,130 @@ def test_needs_no_gradient(fa):
     with torch.no_grad():
         out = fa.forward_packed(q, q, q, cu)
     assert not out.requires_grad and math.isfinite(float(out.float().sum()))
+
+
+# few rows over many keys: the keys of a row are dealt to several workgroups
+CUT_CASES = [
+    ([130], [4200], 2, 1, 128, BF16),
+    ([300, 40], [2600, 1500], 4, 2, 64, F16),
+    ([5, 64, 300], [700, 129, 3001], 6, 2, 128, F16),
+    ([1], [9000], 2, 1, 72, BF16),
+    ([1, 0, 1, 200], [1024, 77, 0, 2047], 4, 1, 96, F16),
+    ([2500], [2500], 2, 1, 64, BF16),
+    ([1500], [1100], 2, 2, 128, BF16),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", CUT_CASES, ids=lambda c: f"q{'-'.join(map(str, c[0]))}_k{'-'.join(map(str, c[1]))}_{c[2]}x{c[3]}_d{c[4]}_{str(c[5])[6:]}")
+def test_few_rows_over_many_keys(fa, case, causal):
+    q_lens, k_lens, hq, hk, d, dtype = case
+    q, k, v, _ = make(q_lens, k_lens, hq, hk, d, dtype, seed=sum(k_lens))
+    got = call(fa, q, k, v, q_lens, k_lens, causal=causal)
+    ref.check_packed(got, q, k, v, q_lens, k_lens, causal, d ** -0.5, heads=[0, hq - 1])
+    for _ in range(3):
+        assert torch.equal(call(fa, q, k, v, q_lens, k_lens, causal=causal), got)
+
+
+def _packed_args(q, k, v, out, cu_q, cu_k, causal=True):
+    import ctypes
+
+    class Packed(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "cu_q", "cu_k")] +
+                    [(n, ctypes.c_int64) for n in ("sequences", "total_q", "total_k", "q_heads", "kv_heads", "d", "qt", "qh", "kt", "kh", "vt", "vh", "ot", "oh")] +
+                    [("softmax_scale", ctypes.c_float), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32)])
+    strides = [s for x in (q, k, v, out) for s in x.stride()[:2]]
+    return Packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), len(cu_q) - 1, q.shape[0], k.shape[0],
+                  q.shape[1], k.shape[1], q.shape[2], *strides, q.shape[2] ** -0.5, int(causal), {F16: 0, BF16: 1}[q.dtype])
+
+
+def test_cut_with_a_workspace_and_whole_without(fa):
+    """Through the C entry: one workspace, whose parts hold NaN in front of each call, for calls of several shapes; and none."""
+    import ctypes
+    L = fa.lib()
+    work = torch.zeros(1 << 26, dtype=torch.uint8, device="cuda")
+    for q_lens, k_lens, hq, hk, d, dtype in CUT_CASES[:4]:
+        q, k, v, _ = make(q_lens, k_lens, hq, hk, d, dtype, seed=3)
+        dev = [x.cuda() for x in (q, k, v)] + [torch.full_like(q, 5.0).cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda()]
+        a = _packed_args(*dev)
+        need = L.flash_fwd_packed_workspace_bytes(ctypes.byref(a))
+        assert need > 2048
+        assert need <= work.numel()
+        work[2048:] = 255               # (an earlier call may have needed more)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert L.flash_fwd_packed(ctypes.byref(a), work.data_ptr(), need, stream) == 0, L.flash_hip_last_error()
+        torch.cuda.synchronize()
+        assert not bool(work[:2048].any())
+        assert bool((work[need:] == 255).all())
+        ref.check_packed(dev[3], q, k, v, q_lens, k_lens, True, d ** -0.5, heads=[0])
+        dev[3].fill_(5.0)
+        assert L.flash_fwd_packed(ctypes.byref(a), None, 0, stream) == 0, L.flash_hip_last_error()
+        ref.check_packed(dev[3], q, k, v, q_lens, k_lens, True, d ** -0.5, heads=[0])
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf"), "lowest"])
+def test_cut_rows_and_masked_places(fa, poison):
+    """As test_masked_places_may_hold_anything, with the diagonal in the last of several parts, and values in the first
+    part that every row sees."""
+    nq, nk, d = 150, 2300, 128
+    q, k, v, _ = make([nq], [nk], 2, 1, d, BF16, seed=21)
+    bad = torch.finfo(BF16).min if poison == "lowest" else poison
+    for row in (nk - 149, nk - 70, nk - 3):
+        v[row, 0, 3::7] = bad
+    got = call(fa, q, k, v, [nq], [nk])
+    ref.check_packed(got, q, k, v, [nq], [nk], True, d ** -0.5)
+    k[nk - 1] = bad
+    got2 = call(fa, q, k, v, [nq], [nk])
+    assert torch.equal(got2[:nq - 1].view(torch.int16), got[:nq - 1].view(torch.int16))
+    v[100, 0, 5] = bad
+    k[nk - 1] = 0.0
+    got = call(fa, q, k, v, [nq], [nk])
+    ref.check_packed(got, q, k, v, [nq], [nk], True, d ** -0.5)
+
+
+def test_cut_rows_in_a_graph_beside_eager_calls(fa):
+    """A captured call has scratch of its own: replays on one stream beside eager calls, and another graph, on others."""
+    hq, hk, d, total_q, total_k = 4, 2, 64, 260, 4000
+    q, k, v, _ = make([total_q], [total_k], hq, hk, d, F16, seed=22)
+    qd, kd, vd = q.cuda(), k.cuda(), v.cuda()
+    cu_q, cu_k = ref.offsets([130, 130]).cuda(), ref.offsets([2000, 2000]).cuda()
+    outs = [torch.empty_like(qd) for _ in range(3)]
+    sides = [torch.cuda.Stream() for _ in range(3)]
+    graphs = []
+    torch.cuda.synchronize()
+    for out, side in zip(outs[:2], sides):
+        with torch.cuda.stream(side):
+            fa.forward_packed(qd, kd, vd, cu_q, cu_k, out=out, sync=False)
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                fa.forward_packed(qd, kd, vd, cu_q, cu_k, out=out, sync=False)
+        graphs.append(graph)
+    for q_lens, k_lens in (([130, 130], [2000, 2000]), ([260, 0], [3000, 1000]), ([3, 257], [10, 3990])):
+        cu_q.copy_(ref.offsets(q_lens))
+        cu_k.copy_(ref.offsets(k_lens))
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, side in zip(graphs, sides):
+                with torch.cuda.stream(side):
+                    graph.replay()
+            with torch.cuda.stream(sides[2]):
+                fa.forward_packed(qd, kd, vd, cu_q, cu_k, out=outs[2], sync=False)
+        torch.cuda.synchronize()
+        for out in outs:
+            assert torch.equal(out, outs[0])
+        ref.check_packed(outs[0], q, k, v, q_lens, k_lens, True, d ** -0.5, heads=[0, 3])
+
+
+@pytest.mark.parametrize("d,dtype,causal", [(128, BF16, True), (64, F16, False), (40, BF16, True)])
+def test_rows_far_apart(fa, d, dtype, causal):
+    """Rows more than 4 MiB apart (one row of a wide array per token)."""
+    q_lens, k_lens = [5, 70], [40, 130]
+    q, k, v, _ = make(q_lens, k_lens, 2, 1, d, dtype, seed=23)
+    wide = torch.zeros(sum(k_lens), (1 << 21) + 64, dtype=dtype, device="cuda")
+    kd = wide[:, :d].unflatten(1, (1, d))
+    kd.copy_(k)
+    got = fa.forward_packed(q.cuda(), kd, v.cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda(), causal=causal)
+    ref.check_packed(got, q, k, v, q_lens, k_lens, causal, d ** -0.5)

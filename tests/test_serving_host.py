@@ -227,7 +227,18 @@ def test_packed_refusals_through_the_abi(fa):
                           (dict(oh=-64), "negative"), (dict(dtype=2), "float16"), (dict(causal=2), "causal"), (dict(d=52), "head dim"),
                           (dict(q_heads=5), "multiple"), (dict(total_q=-1), "between"), (dict(total_k=1 << 31), "between"), (dict(softmax_scale=0.0), "softmax_scale")):
         p = Packed(**{**good, **change})
-        assert refused(fa, L.flash_fwd_packed(ctypes.byref(p), None), match), change
-    assert refused(fa, L.flash_fwd_packed(None, None), "null")
-    assert L.flash_fwd_packed(ctypes.byref(Packed(**{**good, "sequences": 0, "q": None})), None) == 0
-    assert L.flash_fwd_packed(ctypes.byref(Packed(**{**good, "total_q": 0, "q": None})), None) == 0
+        assert refused(fa, L.flash_fwd_packed(ctypes.byref(p), None, 0, None), match), change
+    # a workspace, where one is of use: few rows over many keys
+    few = Packed(**{**good, "total_k": 4096})
+    need = L.flash_fwd_packed_workspace_bytes(ctypes.byref(few))
+    assert need > 2048
+    assert refused(fa, L.flash_fwd_packed(ctypes.byref(few), P, need - 1, None), "too small")
+    assert refused(fa, L.flash_fwd_packed(ctypes.byref(few), P + 8, need, None), "aligned")
+    assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(Packed(**good))) == 0                                     # few keys
+    assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(Packed(**{**good, "total_k": 4096, "total_q": 1 << 20}))) == 0  # many rows
+    assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(Packed(**{**good, "total_q": 0}))) == 0
+    assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(Packed(**{**good, "d": 52}))) == -1
+    assert L.flash_fwd_packed_workspace_bytes(None) == -1
+    assert refused(fa, L.flash_fwd_packed(None, None, 0, None), "null")
+    assert L.flash_fwd_packed(ctypes.byref(Packed(**{**good, "sequences": 0, "q": None})), None, 0, None) == 0
+    assert L.flash_fwd_packed(ctypes.byref(Packed(**{**good, "total_q": 0, "q": None})), None, 0, None) == 0
