@@ -31,10 +31,13 @@ using DiagonalPlan = TilePlan<T % kPeriod, T, (T + 1 < kQ16 ? T + 1 : T), (T > 0
 
 // A part of an item: the tiles [first, behind) of its keys.  SPLIT kernels cut items with many tiles where there are too few
 // of them to fill the chip: every part leaves its sums, and the last one to do so adds them up.
-constexpr int kMostParts = 4, kPartTiles = 8;  // parts of an item at most, tiles of a part at least
+constexpr int kMostParts = 16, kPartTiles = 8;  // parts of an item at most, tiles of a part at least
 struct Part {
   int parts, first, behind;
 };
+// Item of workgroup `place` of those that work on part `nth` (workgroup i runs on XCD i % 8, and there are a multiple of 8
+// items): the parts of an item go to different XCDs.
+__device__ __forceinline__ uint32_t item_of_part(uint32_t place, uint32_t nth) { return place ^ (nth & 7u); }
 template <int D, typename TO, bool CAUSAL, bool SPLIT>
 __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Item item, const Part& part, char* smem_raw);
 
@@ -46,7 +49,7 @@ __global__ __launch_bounds__(kThreads, kQ16 == 2 ? 2 : 1) void attn_fwd_kernel_p
   {
     Part part{1, 0, 0};
     const uint32_t nth = SPLIT ? blockIdx.x / p.items : 0;  // number of the part
-    const packed::Item item = packed::find_item(p, SPLIT ? blockIdx.x - nth * p.items : blockIdx.x, kPackedRows, CAUSAL, (int)(threadIdx.x & 63));
+    const packed::Item item = packed::find_item(p, SPLIT ? item_of_part(blockIdx.x - nth * p.items, nth) : blockIdx.x, kPackedRows, CAUSAL, (int)(threadIdx.x & 63));
     if (!item.it.there) return;
     // rows that see no key: at most the first ones of a sequence with more queries than keys
     again = item.it.nk == 0 || item.a0 < 0;
@@ -70,7 +73,7 @@ __global__ __launch_bounds__(kThreads, kQ16 == 2 ? 2 : 1) void attn_fwd_kernel_p
     asm volatile("" : "+s"(late));
     int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     asm volatile("" : "+v"(lane));
-    const packed::Item item = packed::find_item(*late, SPLIT ? blockIdx.x % late->items : blockIdx.x, kPackedRows, CAUSAL, lane);
+    const packed::Item item = packed::find_item(*late, SPLIT ? item_of_part(blockIdx.x % late->items, blockIdx.x / late->items) : blockIdx.x, kPackedRows, CAUSAL, lane);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 #pragma unroll 1
     for (int q = 0; q < kQ16; ++q) {
@@ -379,7 +382,7 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
     __builtin_amdgcn_raw_buffer_store_b128(out, o_rs, off, 0, 0);
     if constexpr (CAUSAL) odd |= there && packed::holds_not_finite<EK == kBF16>(out);
   };
-  if (!SPLIT || part.parts == 1) {
+  if (!SPLIT || __builtin_expect(part.parts == 1, 1)) {  // (expected: else O^T moves to other registers here, and spills)
 #pragma unroll
     for (int q = 0; q < kQ16; ++q) {
       const float inv = __builtin_amdgcn_rcpf(quad_lane_sum(lsum[q][0], lane_e));
@@ -394,13 +397,14 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
     // (the arguments are read again here, rather than kept in registers through the iterations)
     const packed::Params* late = (const packed::Params*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(late));
-    const uint32_t nth = blockIdx.x / late->items, number = blockIdx.x - nth * late->items;
+    const uint32_t nth = blockIdx.x / late->items, number = item_of_part(blockIdx.x - nth * late->items, nth);
     const uint32_t slots = late->items * (uint32_t)late->parts;
     const __amdgpu_buffer_rsrc_t part_o = __builtin_amdgcn_make_buffer_rsrc(late->part_o, 0, (int)(slots * kPartFloats * 4u), 0x00020000);
     const __amdgpu_buffer_rsrc_t part_ml = __builtin_amdgcn_make_buffer_rsrc(late->part_ml, 0, (int)(slots * (uint32_t)kPackedRows * 8u), 0x00020000);
     const uint32_t slot0 = number * (uint32_t)late->parts;
+    // (a scalar: byte offset of the wave's values in a part)
     auto o_at = [&](uint32_t slot, int q, int b) __attribute__((always_inline)) {
-      return (slot * kPartFloats + (uint32_t)((((wave * kQ16 + q) * kDv16 + b) * 64 + lane_e) * 4)) * 4u;
+      return (int)((slot * kPartFloats + (uint32_t)(((wave * kQ16 + q) * kDv16 + b) * 64 * 4)) * 4u);
     };
     auto ml_at = [&](uint32_t slot, int q) __attribute__((always_inline)) {
       return (slot * (uint32_t)kPackedRows + (uint32_t)(64 * q + 16 * wave + n_e)) * 8u;
@@ -410,7 +414,7 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
       const float l = quad_lane_sum(lsum[q][0], lane_e);
 #pragma unroll
       for (int b = 0; b < kDv16; ++b) {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[q][b]), part_o, o_at(slot0 + nth, q, b), 0, kThrough);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[q][b]), part_o, lane_e * 16, o_at(slot0 + nth, q, b), kThrough);
       }
       if (g_e == 0) {
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(st[q].mc * sc.c), __float_as_uint(l)}, part_ml,
@@ -425,45 +429,51 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
     if (*said != (uint32_t)part.parts - 1) return false;
     asm volatile("" ::: "memory");
     if (tid == 0) __hip_atomic_store(late->tickets + number, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int parts = part.parts;
+    // reference and sum of a row in part `first` + g_e, or in the last part
+    auto load_ml = [&](int q, int first) __attribute__((always_inline)) {
+      const int i = first + g_e < parts ? first + g_e : parts - 1;
+      return __builtin_amdgcn_raw_buffer_load_b64(part_ml, ml_at(slot0 + (uint32_t)i, q), 0, kThrough);
+    };
 #pragma unroll 1
     for (int q = 0; q < kQ16; ++q) {
-      float w[kMostParts], l = 0.f, m = -INFINITY;
-      u32x2 ml[kMostParts];
-#pragma unroll
-      for (int i = 0; i < kMostParts; ++i) {
-        ml[i] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, ml_at(slot0 + (uint32_t)(i < part.parts ? i : part.parts - 1), q), 0, kThrough);
-      }
-#pragma unroll
-      for (int i = 0; i < kMostParts; ++i) m = fmaxf(m, __uint_as_float(ml[i][0]));
-#pragma unroll
-      for (int i = 0; i < kMostParts; ++i) {
-        w[i] = i < part.parts ? fast_exp2(__uint_as_float(ml[i][0]) - m) : 0.f;
-        l += i < part.parts ? w[i] * __uint_as_float(ml[i][1]) : 0.f;
-      }
-      const float inv = __builtin_amdgcn_rcpf(l);
-      constexpr int kTogether = 4;  // tiles of O^T whose parts are fetched together
-#pragma unroll
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int first = 0; first < parts; first += 4) m = fmaxf(m, __uint_as_float(load_ml(q, first)[0]));
+      m = quad_lane_max(m, lane_e);
+      constexpr int kTogether = 4;  // tiles of O^T that are fetched together, of four parts
+#pragma unroll 1
       for (int b0 = 0; b0 < kDv16; b0 += kTogether) {
-        f32x4 x[kTogether][kMostParts];
+        f32x4 sum[kTogether];
+        float l = 0.f;
 #pragma unroll
-        for (int b = 0; b < kTogether; ++b) {
+        for (int b = 0; b < kTogether; ++b) sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int first = 0; first < parts; first += 4) {
+          const u32x2 ml = load_ml(q, first);
+          f32x4 x[kTogether][4];
 #pragma unroll
-          for (int i = 0; i < kMostParts; ++i) {
-            x[b][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                    part_o, o_at(slot0 + (uint32_t)(i < part.parts ? i : part.parts - 1), q, b0 + b), 0, kThrough));
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t slot = slot0 + (uint32_t)(first + i < parts ? first + i : parts - 1);
+#pragma unroll
+            for (int b = 0; b < kTogether; ++b) {
+              x[b][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part_o, lane_e * 16, o_at(slot, q, b0 + b), kThrough));
+            }
+          }
+          const float w = first + g_e < parts ? fast_exp2(__uint_as_float(ml[0]) - m) : 0.f;
+          l += first + g_e < parts ? w * __uint_as_float(ml[1]) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float wi = __shfl(w, 16 * i + n_e);
+#pragma unroll
+            for (int b = 0; b < kTogether; ++b) {
+              if (first + i < parts) sum[b] += x[b][i] * wi;
+            }
           }
         }
+        const float inv = __builtin_amdgcn_rcpf(quad_lane_sum(l, lane_e));
 #pragma unroll
-        for (int b = 0; b < kTogether; ++b) {
-          f32x4 sum = x[b][0] * w[0];
-#pragma unroll
-          for (int i = 1; i < kMostParts; ++i) {
-            if (i < part.parts) sum += x[b][i] * w[i];
-          }
-          x[b][0] = sum;
-        }
-#pragma unroll
-        for (int b = 0; b < kTogether; b += 2) store_pair(q, b0 + b, x[b][0], x[b + 1][0], inv);
+        for (int b = 0; b < kTogether; b += 2) store_pair(q, b0 + b, sum[b], sum[b + 1], inv);
       }
     }
   }

@@ -59,8 +59,8 @@ void set_grid(packed::Params& p, int64_t rows) {
   p.parts = 1;
 }
 // Fewer 128-row items than three quarters of the places on the chip (two for each of 256 compute units), with enough keys to
-// cut: the keys of an item are dealt to several workgroups.  Twice the places are aimed at, since the items are not alike and
-// the grid holds some that do not exist.
+// cut: the keys of an item are dealt to several workgroups, as many as fill the places by what there may be of items (the
+// grid holds one more for every sequence and head).
 int parts_of(const packed::Params& p) {
   constexpr int64_t kPlaces = 512;
   if (!take_half(p) || p.total_k < 2 * m16h::kPartTiles * kBc) return 1;
@@ -68,7 +68,7 @@ int parts_of(const packed::Params& p) {
   set_grid(h, m16h::kPackedRows);
   static_assert(kPlaces * 3 / 4 * 4 <= FLASH_PACKED_TICKET_BYTES, "one ticket for each item that is cut");
   if ((int64_t)h.items * 4 >= kPlaces * 3) return 1;
-  const int64_t wanted = 2 * kPlaces / h.items;
+  const int64_t items = (int64_t)(h.tiles - p.sequences) * p.heads, wanted = (kPlaces + items - 1) / items;
   return (int)(wanted < m16h::kMostParts ? wanted : m16h::kMostParts);
 }
 // floats of a part of an item: its rows of O^T, and their reference and sum
