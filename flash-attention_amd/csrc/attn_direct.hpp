@@ -1,5 +1,5 @@
 // One wave's step of attention with K and V taken straight from memory into matrix operands: 32 keys (or 64)
-// against NQ blocks of 16 query rows, no LDS.  The building block of the decoding kernel, where K and V are
+// against 16 query rows, no LDS.  The building block of the decoding kernel, where K and V are
 // read once and never shared between waves.
 //
 // Mathematics, per query (column) q and key j, in the exp2 domain (c = softmax_scale * log2 e):
@@ -126,8 +126,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
   return x;
 }
 
-// D: head dim rounded up to 64 or 128; CACHE8: K and V are e4m3; NS: 32-key blocks per step; NQ: 16-query blocks
-template <int D, int EK, bool CACHE8, int NS, int NQ>
+// D: head dim rounded up to 64 or 128; CACHE8: K and V are e4m3; NS: 32-key blocks per step
+template <int D, int EK, bool CACHE8, int NS>
 struct Step {
   static constexpr int kKS = D / 32;             // k-steps of a score tile
   static constexpr int kE = D / 16;              // columns of V per lane
@@ -141,18 +141,15 @@ struct Step {
   typedef VWord VBlock[NS][8];
 
   struct State {
-    f32x4 o[NQ][kE];
-    float m[NQ], l[NQ];  // l: this lane's keys only
+    f32x4 o[kE];
+    float m, l;  // l: this lane's keys only
   };
 
   static __device__ __forceinline__ void clear(State& st) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) st.o[q][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-      st.m[q] = kMinusInf;
-      st.l[q] = 0.f;
-    }
+    for (int e = 0; e < kE; ++e) st.o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    st.m = kMinusInf;
+    st.l = 0.f;
   }
 
   // first of the 8 head-dim elements that lane group g multiplies in k-step ks; a 16-byte load of an 8-bit row holds
@@ -201,89 +198,85 @@ struct Step {
   // `c`: softmax scale * log2 e (and what a unit of an 8-bit K stands for).  `valid`: bit i: key i of the step exists
   // (wave-uniform).  LIMIT: the lane's query sees the first `limit` keys of the step only (fewer than one: none).
   struct Weights {
-    u32x4 hi[NQ][NS], lo[NQ][NS];
+    u32x4 hi[NS], lo[NS];
     float p[2 * NS][4];  // as computed (LIMIT only)
   };
   template <bool LIMIT>
-  static __device__ __forceinline__ void weigh(State& st, Weights& w, const KBlock& k, const u32x4 (&qf)[NQ][kKS], uint64_t valid, float c,
+  static __device__ __forceinline__ void weigh(State& st, Weights& w, const KBlock& k, const u32x4 (&qf)[kKS], uint64_t valid, float c,
                                                int lane, int limit = kKeys) {
     const int g = lane >> 4;
     constexpr uint64_t kAll = NS == 1 ? 0xffffffffull : ~0ull;
-    f32x4 s[NQ][2 * NS];
+    f32x4 s[2 * NS];
 #pragma unroll
     for (int t = 0; t < 2 * NS; ++t) {
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) {
         const u32x4 a = k_operand(k[t], ks);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) s[q][t] = mfma<EK>(a, qf[q][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[q][t]);
+        s[t] = mfma<EK>(a, qf[ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[t]);
       }
     }
     const bool cut = LIMIT && __builtin_amdgcn_ballot_w64(limit < kKeys) != 0;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int t = 0; t < 2 * NS; ++t) s[q][t] *= c;
-      if (valid != kAll) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const uint32_t mine = lane_bits(valid, n, g);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (!((mine >> (16 * t + i)) & 1)) s[q][2 * n + t][i] = kMinusInf;
-            }
-          }
-        }
-      }
-      if constexpr (LIMIT) {
-        if (cut) {
-#pragma unroll
-          for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (16 * t + 4 * g + i >= limit) s[q][t][i] = kMinusInf;
-            }
-          }
-        }
-      }
-      float mx = s[q][0][0];
-#pragma unroll
-      for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][t][i]);
-      }
-      const float m_new = fmaxf(st.m[q], quad_max(mx));
-      // nothing visible so far: any finite reference will do (every p is 0)
-      const float ref = m_new == kMinusInf ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(st.m[q] - ref);
-      st.m[q] = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2 * NS; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[q][t][i] = __builtin_amdgcn_exp2f(s[q][t][i] - ref);
-          sum += s[q][t][i];
-          if constexpr (LIMIT) w.p[t][i] = s[q][t][i];
-        }
-      }
-      st.l[q] = st.l[q] * alpha + sum;
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
-#pragma unroll
-        for (int e = 0; e < kE; ++e) st.o[q][e] *= alpha;
-      }
+    for (int t = 0; t < 2 * NS; ++t) s[t] *= c;
+    if (valid != kAll) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
+        const uint32_t mine = lane_bits(valid, n, g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = s[q][2 * n + i / 2][2 * (i & 1)], y = s[q][2 * n + i / 2][2 * (i & 1) + 1];
-          w.hi[q][n][i] = pack2<EK>(x, y);
-          if constexpr (!LIMIT) {
-            const f32x2 back = unpack2<EK>(w.hi[q][n][i]);
-            w.lo[q][n][i] = pack2<EK>(x - back[0], y - back[1]);
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!((mine >> (16 * t + i)) & 1)) s[2 * n + t][i] = kMinusInf;
           }
+        }
+      }
+    }
+    if constexpr (LIMIT) {
+      if (cut) {
+#pragma unroll
+        for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (16 * t + 4 * g + i >= limit) s[t][i] = kMinusInf;
+          }
+        }
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+    }
+    const float m_new = fmaxf(st.m, quad_max(mx));
+    // nothing visible so far: any finite reference will do (every p is 0)
+    const float ref = m_new == kMinusInf ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(st.m - ref);
+    st.m = m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * NS; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+        sum += s[t][i];
+        if constexpr (LIMIT) w.p[t][i] = s[t][i];
+      }
+    }
+    st.l = st.l * alpha + sum;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) st.o[e] *= alpha;
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = s[2 * n + i / 2][2 * (i & 1)], y = s[2 * n + i / 2][2 * (i & 1) + 1];
+        w.hi[n][i] = pack2<EK>(x, y);
+        if constexpr (!LIMIT) {
+          const f32x2 back = unpack2<EK>(w.hi[n][i]);
+          w.lo[n][i] = pack2<EK>(x - back[0], y - back[1]);
         }
       }
     }
@@ -328,11 +321,8 @@ struct Step {
       for (int i = 0; i < 4; ++i) {
         a[i] = __builtin_amdgcn_perm(r[2 * i + 1][e / 2], r[2 * i][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
       }
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        if constexpr (HIGH) st.o[q][e] = mfma<EK>(a, w.hi[q][n], st.o[q][e]);
-        if constexpr (LOW) st.o[q][e] = mfma<EK>(a, w.lo[q][n], st.o[q][e]);
-      }
+      if constexpr (HIGH) st.o[e] = mfma<EK>(a, w.hi[n], st.o[e]);
+      if constexpr (LOW) st.o[e] = mfma<EK>(a, w.lo[n], st.o[e]);
     }
   }
 
@@ -357,12 +347,9 @@ struct Step {
   static __device__ __forceinline__ bool holds_nan(const State& st) {
     bool any = false;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
+    for (int e = 0; e < kE; ++e) {
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) any |= st.o[q][e][i] != st.o[q][e][i];
-      }
+      for (int i = 0; i < 4; ++i) any |= st.o[e][i] != st.o[e][i];
     }
     return __builtin_amdgcn_ballot_w64(any) != 0;
   }
@@ -370,7 +357,6 @@ struct Step {
   // o += p v, p rounded once, for keys that some of the 16 queries see and others do not: 0 * infinity in the product
   // would reach those that do not.  Such values go around it, to the queries that see them only.
   static __device__ __forceinline__ void accumulate_limited(State& st, const Weights& w, const VBlock& v, int lane, int limit) {
-    static_assert(NQ == 1, "one limit per lane");
     const int n16 = lane & 15, g = lane >> 4;
     const bool cut = __builtin_amdgcn_ballot_w64(limit < kKeys) != 0;
 #pragma unroll
@@ -401,8 +387,8 @@ struct Step {
                 for (int c = 0; c < kE / 2; ++c) {
                   const uint32_t x = (uint32_t)__shfl((int)r[j][c], 16 * from + 4 * g + i);
                   const f32x2 y = unpack2<EK>(x);
-                  if (sees && not_finite(x)) st.o[0][2 * c][i] += p * y[0];
-                  if (sees && not_finite(x >> 16)) st.o[0][2 * c + 1][i] += p * y[1];
+                  if (sees && not_finite(x)) st.o[2 * c][i] += p * y[0];
+                  if (sees && not_finite(x >> 16)) st.o[2 * c + 1][i] += p * y[1];
                 }
               }
             }

@@ -95,12 +95,12 @@ struct TileLine {
 template <int D, int EK, bool FULL>
 __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int32_t row0, int32_t head, int lane) {
   using namespace direct;
-  using S = Step<D, EK, false, 1, 1>;
+  using S = Step<D, EK, false, 1>;
   if (row0 >= t.nq || row0 + 15 < 0) return;
   const int n = lane & 15, g = lane >> 4;
   const int32_t kvh = head / (p.heads / p.kv_heads);
   const int32_t row = row0 + n;
-  u32x4 qf[1][S::kKS];
+  u32x4 qf[S::kKS];
   const bool mine = (uint32_t)row < (uint32_t)t.nq;
   const char* src = p.q + (int64_t)(t.q0 + (mine ? row : 0)) * p.q_token + (int64_t)head * p.q_head;
 #pragma unroll
@@ -108,7 +108,7 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
     const int col = S::column(ks, g);
     const bool there = mine && (FULL || col < p.d);
     const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
-    qf[0][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
+    qf[ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
   }
   // keys the lane's query sees, and those the last row of the 16 does
   const int32_t sees = visible_keys(row, t.nq, t.nk, p.causal);
@@ -144,7 +144,7 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
     S::template weigh<true>(st, w, k, qf, valid, p.scale_log2, lane, sees - key0);
     S::accumulate_limited(st, w, v, lane, sees - key0);
   }
-  const float l = quad_sum(st.l[0]);
+  const float l = quad_sum(st.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (!mine) return;
   char* dst = p.o + (int64_t)(t.q0 + row) * p.o_token + (int64_t)head * p.o_head;
@@ -154,10 +154,10 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
     if (FULL || col < p.d) {
       typename S::VWord w;
       if constexpr (S::kE == 8) {
-        w = u32x4{pack2<EK>(st.o[0][0][i] * inv, st.o[0][1][i] * inv), pack2<EK>(st.o[0][2][i] * inv, st.o[0][3][i] * inv),
-                  pack2<EK>(st.o[0][4][i] * inv, st.o[0][5][i] * inv), pack2<EK>(st.o[0][6][i] * inv, st.o[0][7][i] * inv)};
+        w = u32x4{pack2<EK>(st.o[0][i] * inv, st.o[1][i] * inv), pack2<EK>(st.o[2][i] * inv, st.o[3][i] * inv),
+                  pack2<EK>(st.o[4][i] * inv, st.o[5][i] * inv), pack2<EK>(st.o[6][i] * inv, st.o[7][i] * inv)};
       } else {
-        w = u32x2{pack2<EK>(st.o[0][0][i] * inv, st.o[0][1][i] * inv), pack2<EK>(st.o[0][2][i] * inv, st.o[0][3][i] * inv)};
+        w = u32x2{pack2<EK>(st.o[0][i] * inv, st.o[1][i] * inv), pack2<EK>(st.o[2][i] * inv, st.o[3][i] * inv)};
       }
       *(typename S::VWord*)(dst + col * 2) = w;
     }

@@ -38,8 +38,8 @@ struct Params {
   const int32_t* lens;
   const float* k_scale;  // per K/V head, null: 1
   const float* v_scale;
-  float* part_o;         // [2 * workgroups][16 * NQ][D]
-  float* part_ml;        // [2 * workgroups][16 * NQ][2]
+  float* part_o;         // [2 * workgroups][16][D]
+  float* part_ml;        // [2 * workgroups][16][2]
   uint32_t* tickets;     // one for each triple; zero, and left zero
   int64_t q_batch, q_head, o_batch, o_head;     // bytes
   Pages pages;                                   // K and V alike
@@ -47,7 +47,7 @@ struct Params {
   int64_t table_stride;                          // entries
   int32_t batch, kv_heads, group;                // group: query heads per K/V head
   int32_t d;
-  int32_t qblocks;                               // blocks of 16 * NQ query heads per K/V head
+  int32_t qblocks;                               // blocks of 16 query heads per K/V head
   uint32_t workgroups;
   float scale_log2;                              // softmax scale * log2 e
 };
@@ -68,27 +68,27 @@ __device__ __forceinline__ T stream(const T* p) {
   return __builtin_nontemporal_load(p);
 }
 
-template <int D, int EK, bool CACHE8, int NQ, bool FULL, bool PAGE16>
+template <int D, int EK, bool CACHE8, bool FULL, bool PAGE16>
 __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NS = kSub<D, CACHE8>;
   constexpr int kUnitKeys = kUnit<D, CACHE8>;
-  using S = Step<D, EK, CACHE8, NS, NQ>;
+  using S = Step<D, EK, CACHE8, NS>;
   constexpr int kRowFloats = D + 4;  // rows of the waves' sums, shifted by four banks each
   // the waves' sums; later the weights of a triple's parts (at most `workgroups` of them, for 8 rows)
   constexpr int kShFloats = kWaves * 16 * kRowFloats > 8 * kMostWorkgroups ? kWaves * 16 * kRowFloats : 8 * kMostWorkgroups;
   __shared__ __attribute__((aligned(16))) float sh[kShFloats];
   __shared__ __attribute__((aligned(16))) f32x4 sh_sum[kThreads];
-  __shared__ float sh_ml[kWaves][NQ * 16][2];
+  __shared__ float sh_ml[kWaves][16][2];
   __shared__ float sh_l[8];
   __shared__ uint32_t sh_ticket;
   float(&sh_o)[kWaves][16][kRowFloats] = *(float(*)[kWaves][16][kRowFloats]) & sh[0];
 
   // Parts go to memory and come from there past the L2s, which the XCDs do not share (sc0 sc1: system scope).  A release
-  // and an acquire at agent scope write back and drop whole L2s instead: 174 us where this takes 66 (32 ragged sequences).
+  // and an acquire at agent scope write back and drop whole L2s instead: 174 us where this takes 63 (32 ragged sequences).
   constexpr int kThrough = 17;
-  const __amdgpu_buffer_rsrc_t part_o = __builtin_amdgcn_make_buffer_rsrc(p.part_o, 0, (int)(p.workgroups * 2u * 16u * NQ * D * 4u), 0x00020000);
-  const __amdgpu_buffer_rsrc_t part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, (int)(p.workgroups * 2u * 16u * NQ * 8u), 0x00020000);
+  const __amdgpu_buffer_rsrc_t part_o = __builtin_amdgcn_make_buffer_rsrc(p.part_o, 0, (int)(p.workgroups * 2u * 16u * D * 4u), 0x00020000);
+  const __amdgpu_buffer_rsrc_t part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, (int)(p.workgroups * 2u * 16u * 8u), 0x00020000);
 
   const int lane = threadIdx.x & 63;
   const int wave = (int)uniform(threadIdx.x >> 6);
@@ -130,22 +130,18 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     const uint32_t left = r_end - r;
     const uint32_t u1 = units - u0 < left ? units : u0 + left;
     const int32_t kvh = (int32_t)(vh / (uint32_t)p.qblocks), qb = (int32_t)(vh - (uint32_t)(kvh * p.qblocks));
-    const int32_t row0 = qb * (16 * NQ);                                // first query head inside the group
-    const int32_t rows = p.group - row0 < 16 * NQ ? p.group - row0 : 16 * NQ;
+    const int32_t row0 = qb * 16;  // first query head inside the group
+    const int32_t rows = p.group - row0 < 16 ? p.group - row0 : 16;
 
     // queries of the block, zeros for the heads that do not exist
-    u32x4 qf[NQ][S::kKS];
+    u32x4 qf[S::kKS];
+    const char* src = p.q + (int64_t)b * p.q_batch + (int64_t)(kvh * p.group + row0 + (n < rows ? n : 0)) * p.q_head;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int row = 16 * q + n;
-      const char* src = p.q + (int64_t)b * p.q_batch + (int64_t)(kvh * p.group + row0 + (row < rows ? row : 0)) * p.q_head;
-#pragma unroll
-      for (int ks = 0; ks < S::kKS; ++ks) {
-        const int col = S::column(ks, g);
-        const bool there = row < rows && (FULL || col < p.d);
-        const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
-        qf[q][ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
-      }
+    for (int ks = 0; ks < S::kKS; ++ks) {
+      const int col = S::column(ks, g);
+      const bool there = n < rows && (FULL || col < p.d);
+      const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
+      qf[ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
     }
     const float sc = p.scale_log2 * (CACHE8 && p.k_scale ? p.k_scale[kvh] : 1.f);
     const char* kh = p.k + (int64_t)kvh * p.head_stride;
@@ -240,62 +236,56 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     // NaN may come from an infinite value (rare: the part is worked out again with care)
     if (S::holds_nan(st)) attend(std::true_type{});
 
-    // ---- the four waves' parts, 16 queries at a time -----------------------------------------------------
+    // ---- the four waves' parts --------------------------------------------------------------------------
     const bool complete = u0 == 0 && u1 == units;
     const uint32_t slot = part_slot(blockIdx.x, c, r - u0);
     const float vs = CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const float l = quad_sum(st.l[q]);
-      if (g == 0) {
-        sh_ml[wave][16 * q + n][0] = st.m[q];
-        sh_ml[wave][16 * q + n][1] = l;
-      }
+    const float l = quad_sum(st.l);
+    if (g == 0) {
+      sh_ml[wave][n][0] = st.m;
+      sh_ml[wave][n][1] = l;
     }
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int e = 0; e < S::kE; e += 4) {
-          *(f32x4*)&sh_o[wave][n][S::kE * (4 * g + i) + e] =
-              f32x4{st.o[q][e][i], st.o[q][e + 1][i], st.o[q][e + 2][i], st.o[q][e + 3][i]};
-        }
+      for (int e = 0; e < S::kE; e += 4) {
+        *(f32x4*)&sh_o[wave][n][S::kE * (4 * g + i) + e] =
+            f32x4{st.o[e][i], st.o[e + 1][i], st.o[e + 2][i], st.o[e + 3][i]};
       }
-      __syncthreads();
-      constexpr int kPieces = D / 4;
-      for (int x = threadIdx.x; x < 16 * kPieces && 16 * q + x / kPieces < rows; x += kThreads) {
-        const int row = x / kPieces, col = 4 * (x % kPieces);
-        if (col < p.d) {
-          float m = kMinusInf;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sh_ml[w][16 * q + row][0]);
-          const float ref = m == kMinusInf ? 0.f : m;
-          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-          float l = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sh_ml[w][16 * q + row][0] - ref);
-            l += f * sh_ml[w][16 * q + row][1];
-            sum += f * *(const f32x4*)&sh_o[w][row][col];
-          }
-          if (complete) {
-            const int32_t head = kvh * p.group + row0 + 16 * q + row;
-            const float inv = l == 0.f ? 0.f : vs / l;
-            *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)head * p.o_head + col * 2) =
-                u32x2{pack2<EK>(sum[0] * inv, sum[1] * inv), pack2<EK>(sum[2] * inv, sum[3] * inv)};
-            if (p.lse && col == 0) {
-              p.lse[(int64_t)b * p.kv_heads * p.group + head] = l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
-            }
-          } else {
-            const uint32_t at = slot * (16 * NQ) + (uint32_t)(16 * q + row);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), part_o, (at * D + (uint32_t)col) * 4u, 0, kThrough);
-            if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, part_ml, at * 8u, 0, kThrough);
-          }
-        }
-      }
-      __syncthreads();
     }
+    __syncthreads();
+    constexpr int kPieces = D / 4;
+    for (int x = threadIdx.x; x < 16 * kPieces && x / kPieces < rows; x += kThreads) {
+      const int row = x / kPieces, col = 4 * (x % kPieces);
+      if (col < p.d) {
+        float m = kMinusInf;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sh_ml[w][row][0]);
+        const float ref = m == kMinusInf ? 0.f : m;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(sh_ml[w][row][0] - ref);
+          l += f * sh_ml[w][row][1];
+          sum += f * *(const f32x4*)&sh_o[w][row][col];
+        }
+        if (complete) {
+          const int32_t head = kvh * p.group + row0 + row;
+          const float inv = l == 0.f ? 0.f : vs / l;
+          *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)head * p.o_head + col * 2) =
+              u32x2{pack2<EK>(sum[0] * inv, sum[1] * inv), pack2<EK>(sum[2] * inv, sum[3] * inv)};
+          if (p.lse && col == 0) {
+            p.lse[(int64_t)b * p.kv_heads * p.group + head] = l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
+          }
+        } else {
+          const uint32_t at = slot * 16 + (uint32_t)row;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), part_o, (at * D + (uint32_t)col) * 4u, 0, kThrough);
+          if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, part_ml, at * 8u, 0, kThrough);
+        }
+      }
+    }
+    __syncthreads();
 
     // ---- the last workgroup of a triple to come here adds its parts up, in the line's order
     if (!complete) {
@@ -308,7 +298,7 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
       if (sh_ticket == parts - 1) {
         asm volatile("" ::: "memory");
         if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        auto row_of = [&](uint32_t i, int row) __attribute__((always_inline)) { return part_slot(w0 + i, c, start) * (16 * NQ) + (uint32_t)row; };
+        auto row_of = [&](uint32_t i, int row) __attribute__((always_inline)) { return part_slot(w0 + i, c, start) * 16 + (uint32_t)row; };
         // Loads past the caches take two microseconds: all of them go out together, the first ones of the sums even before
         // the weights are known.  Sums: four columns a thread; with few rows the parts are dealt to `sides` groups of
         // threads, TOGETHER parts a thread at a time.  (Indexes behind the last part read it again.)

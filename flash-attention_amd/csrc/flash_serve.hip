@@ -106,7 +106,7 @@ constexpr int64_t kPartRows = (int64_t)2 * kDecodeWorkgroups * 16, kPartBytes = 
 static_assert(kPartBytes == FLASH_DECODE_PARTS_BYTES, "include/flash_hip.h names the part of the workspace that need not be zero");
 
 struct DecodePlan {
-  int tile_d, nq;
+  int tile_d;
   uint32_t workgroups;
   int64_t bytes;  // 0: no sequence can be cut
 };
@@ -120,36 +120,31 @@ int plan_decode(const flash_decode_args* a, const flash_paged_cache* c, bool mem
   if (memory && c->sequences > 0) REFUSE_IF(!a->q || !a->o, "null tensor pointer");
   const int64_t group = a->q_heads / c->kv_heads;
   plan->tile_d = c->d <= 64 ? 64 : 128;
-  plan->nq = 1;
   const bool cache8 = c->dtype == FLASH_E4M3;
   const int64_t unit = (plan->tile_d == 64 || cache8) ? flash_hip::paged::kUnit<64, false> : flash_hip::paged::kUnit<128, false>;
   const int64_t reach = c->table_width * c->page_size;
   const int64_t most = reach <= unit ? 1 : (reach + unit - 1) / unit;  // units of a sequence
-  const int64_t triples = c->sequences * c->kv_heads * ((group + 16 * plan->nq - 1) / (16 * plan->nq));
+  const int64_t triples = c->sequences * c->kv_heads * ((group + 15) / 16);
   REFUSE_IF(triples * most >= (int64_t)1 << 31 || c->sequences * a->q_heads >= (int64_t)1 << 31, "batch of %lld sequences is too large", (long long)c->sequences);
   plan->workgroups = (uint32_t)(triples * most < kDecodeWorkgroups ? triples * most : kDecodeWorkgroups);
   plan->bytes = most > 1 && triples > 0 ? kPartBytes + (triples * 4 + 15) / 16 * 16 : 0;
   return FLASH_HIP_OK;
 }
 
-template <int D, int EK, bool CACHE8, int NQ>
+template <int D, int EK, bool CACHE8>
 int launch_decode(const DecodeParams& p, hipStream_t stream) {
   namespace pg = flash_hip::paged;
   const bool page16 = p.pages.page_shift >= 4 && 16 * p.pages.slot_stride < ((int64_t)1 << 31);
-  auto kernel = p.d == D ? (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, true, true> : pg::decode_kernel<D, EK, CACHE8, NQ, true, false>)
-                         : (page16 ? pg::decode_kernel<D, EK, CACHE8, NQ, false, true> : pg::decode_kernel<D, EK, CACHE8, NQ, false, false>);
+  auto kernel = p.d == D ? (page16 ? pg::decode_kernel<D, EK, CACHE8, true, true> : pg::decode_kernel<D, EK, CACHE8, true, false>)
+                         : (page16 ? pg::decode_kernel<D, EK, CACHE8, false, true> : pg::decode_kernel<D, EK, CACHE8, false, false>);
   hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(pg::kThreads), 0, stream, p);
   return launched("flash_decode_paged");
 }
-template <int D, int EK, bool CACHE8>
-int launch_decode(const DecodeParams& p, const DecodePlan& plan, hipStream_t stream) {
-  return launch_decode<D, EK, CACHE8, 1>(p, stream);
-}
 template <int D>
-int launch_decode(const DecodeParams& p, const DecodePlan& plan, int dtype, bool cache8, hipStream_t stream) {
+int launch_decode(const DecodeParams& p, int dtype, bool cache8, hipStream_t stream) {
   using namespace flash_hip::direct;
-  if (dtype == FLASH_F16) return cache8 ? launch_decode<D, kHalf, true>(p, plan, stream) : launch_decode<D, kHalf, false>(p, plan, stream);
-  return cache8 ? launch_decode<D, kBfloat, true>(p, plan, stream) : launch_decode<D, kBfloat, false>(p, plan, stream);
+  if (dtype == FLASH_F16) return cache8 ? launch_decode<D, kHalf, true>(p, stream) : launch_decode<D, kHalf, false>(p, stream);
+  return cache8 ? launch_decode<D, kBfloat, true>(p, stream) : launch_decode<D, kBfloat, false>(p, stream);
 }
 
 // ---- packed prompts -----------------------------------------------------------------------------------------------
@@ -250,12 +245,12 @@ int flash_decode_paged(const flash_decode_args* a, const flash_paged_cache* c, v
   p.kv_heads = (int32_t)c->kv_heads;
   p.group = (int32_t)(a->q_heads / c->kv_heads);
   p.d = (int32_t)c->d;
-  p.qblocks = (p.group + 16 * plan.nq - 1) / (16 * plan.nq);
+  p.qblocks = (p.group + 15) / 16;
   p.workgroups = plan.workgroups;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
   const hipStream_t stream = (hipStream_t)hip_stream;
-  return plan.tile_d == 64 ? launch_decode<64>(p, plan, a->dtype, elem == 1, stream)
-                           : launch_decode<128>(p, plan, a->dtype, elem == 1, stream);
+  return plan.tile_d == 64 ? launch_decode<64>(p, a->dtype, elem == 1, stream)
+                           : launch_decode<128>(p, a->dtype, elem == 1, stream);
 }
 
 int flash_cache_append(const flash_append_args* a, const flash_paged_cache* c, void* hip_stream) {
