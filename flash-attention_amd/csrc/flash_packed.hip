@@ -47,7 +47,7 @@ struct HalfOut<m16::bf16_out> {
 // as many waves.  Shorter ones take the 128-row items, two workgroups to a compute unit, of which one computes while
 // the other starts or ends.  Measured, 128-row / 256-row, us: 32 heads of 128 over 8, 16 x 512 rows 67 / 74, 8 x 1024
 // 88 / 97, 4 x 2048 139 / 141, 2 x 4096 243 / 239, 8192 457 / 442, 16384 1775 / 1719; 32 heads of 64, 8 x 1024 56 / 66,
-// 2 x 4096 152 / 154, 8192 288 / 282; 160 items of 128 rows (16 heads of 64) 45 / 67.
+// 2 x 4096 152 / 154, 8192 288 / 282; 973 rows of 16 heads of 64 45 / 67 (not cut, see parts_of).
 bool take_half(const packed::Params& p) {
   return (int64_t)p.total_k < (int64_t)4096 * p.sequences || (int64_t)p.total_q / m16::kPackedRows * p.heads < 512;
 }
@@ -58,18 +58,22 @@ void set_grid(packed::Params& p, int64_t rows) {
   p.items = (uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads);
   p.parts = 1;
 }
-// Fewer 128-row items than three quarters of the places on the chip (two for each of 256 compute units), with enough keys to
-// cut: the keys of an item are dealt to several workgroups, as many as fill the places by what there may be of items (the
-// grid holds one more for every sequence and head).
+// Fewer 128-row items than compute units, with enough keys to cut: the keys of an item are dealt to several workgroups, as
+// many as fill the chip (two on each of 256 compute units) by what there may be of items (the grid holds one more for every
+// sequence and head).  Measured, cut / whole, us: 128 rows over 32768 keys, 8 heads of 128, 69 / 451; 256 over 8192, 32 heads,
+// 57 / 115; 4096 rows, 4 heads, 41.5 / 60.6; 973 rows of three sequences, 16 heads of 64, 30 / 45; with an item for every
+// compute unit there is nothing to gain: 4096 rows, 8 heads, 64 / 62, 1024 over 8192, 32 heads, 124.6 / 123.
 int parts_of(const packed::Params& p) {
-  constexpr int64_t kPlaces = 512;
+  constexpr int64_t kUnits = 256, kMostSlots = 4 * kUnits;
   if (!take_half(p) || p.total_k < 2 * m16h::kPartTiles * kBc) return 1;
   packed::Params h = p;
   set_grid(h, m16h::kPackedRows);
-  static_assert(kPlaces * 3 / 4 * 4 <= FLASH_PACKED_TICKET_BYTES, "one ticket for each item that is cut");
-  if ((int64_t)h.items * 4 >= kPlaces * 3) return 1;
-  const int64_t items = (int64_t)(h.tiles - p.sequences) * p.heads, wanted = (kPlaces + items - 1) / items;
-  return (int)(wanted < m16h::kMostParts ? wanted : m16h::kMostParts);
+  const int64_t items = (int64_t)(h.tiles - p.sequences) * p.heads;
+  if (items >= kUnits) return 1;
+  const int64_t wanted = (2 * kUnits + items - 1) / items, room = kMostSlots / h.items;
+  static_assert(kMostSlots / 2 * 4 <= FLASH_PACKED_TICKET_BYTES, "a ticket for each item that is cut");
+  const int64_t parts = wanted < room ? wanted : room;
+  return (int)(parts < 1 ? 1 : (parts < m16h::kMostParts ? parts : m16h::kMostParts));
 }
 // floats of a part of an item: its rows of O^T, and their reference and sum
 int64_t part_floats(const packed::Params& p) { return (int64_t)m16h::kPackedRows * ((p.d <= 64 ? 64 : 128) + 2); }

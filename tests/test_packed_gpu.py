@@ -233,6 +233,8 @@ CUT_CASES = [
     ([1, 0, 1, 200], [1024, 77, 0, 2047], 4, 1, 96, F16),
     ([2500], [2500], 2, 1, 64, BF16),
     ([1500], [1100], 2, 2, 128, BF16),
+    ([1900], [1700], 2, 2, 128, BF16),
+    ([333], [3333], 5, 1, 40, F16),
 ]
 
 
