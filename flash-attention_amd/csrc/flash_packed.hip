@@ -51,16 +51,16 @@ struct HalfOut<m16::bf16_out> {
 bool take_half(const packed::Params& p) {
   return (int64_t)p.total_k < (int64_t)4096 * p.sequences || (int64_t)p.total_q / m16::kPackedRows * p.heads < 512;
 }
-// The grid's tiles: a sequence has at most two more than whole ones among its rows (its first one may be short, and its
-// last one).
+// The grid's tiles: a sequence has at most two more than whole ones among its rows, its last one and, where its numbers of
+// queries and keys differ and the diagonal is cut, its first one.
 void set_grid(packed::Params& p, int64_t rows) {
-  p.tiles = (uint32_t)(p.total_q / rows + 2 * p.sequences);
+  p.extra = p.causal && !(p.cu_q == p.cu_k && p.total_q == p.total_k) ? 2 : 1;
+  p.tiles = (uint32_t)(p.total_q / rows + (int64_t)p.extra * p.sequences);
   p.items = (uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads);
   p.parts = 1;
 }
 // Fewer 128-row items than compute units, with enough keys to cut: the keys of an item are dealt to several workgroups, as
-// many as fill the chip (two on each of 256 compute units) by what there may be of items (the grid holds one more for every
-// sequence and head).  Measured, cut / whole, us: 128 rows over 32768 keys, 8 heads of 128, 69 / 451; 256 over 8192, 32 heads,
+// many as fill the chip (two on each of 256 compute units) by what there may be of items.  Measured, cut / whole, us: 128 rows over 32768 keys, 8 heads of 128, 69 / 451; 256 over 8192, 32 heads,
 // 57 / 115; 4096 rows, 4 heads, 41.5 / 60.6; 973 rows of three sequences, 16 heads of 64, 30 / 45; with an item for every
 // compute unit there is nothing to gain: 4096 rows, 8 heads, 64 / 62, 1024 over 8192, 32 heads, 124.6 / 123.
 int parts_of(const packed::Params& p) {
@@ -68,7 +68,7 @@ int parts_of(const packed::Params& p) {
   if (!take_half(p) || p.total_k < 2 * m16h::kPartTiles * kBc) return 1;
   packed::Params h = p;
   set_grid(h, m16h::kPackedRows);
-  const int64_t items = (int64_t)(h.tiles - p.sequences) * p.heads;
+  const int64_t items = ((int64_t)p.total_q / m16h::kPackedRows + p.sequences) * p.heads;
   if (items >= kUnits) return 1;
   const int64_t wanted = (2 * kUnits + items - 1) / items, room = kMostSlots / h.items;
   static_assert(kMostSlots / 2 * 4 <= FLASH_PACKED_TICKET_BYTES, "a ticket for each item that is cut");

@@ -151,6 +151,7 @@ int launch_decode(const DecodeParams& p, int dtype, bool cache8, hipStream_t str
 template <int D, int EK>
 int launch_packed_direct(flash_hip::packed::Params p, hipStream_t stream) {
   namespace pk = flash_hip::packed;
+  p.extra = 1;
   p.tiles = (uint32_t)(p.total_q / pk::kDirectRows + p.sequences);
   const dim3 grid(p.tiles, (uint32_t)p.heads);
   if (p.d == D) {

@@ -24,6 +24,11 @@ FLASH_INDEX Range sequence_rows(int32_t from, int32_t to, int32_t total) {
   const int32_t start = within(from, 0, total);
   return Range{start, within(to, start, total) - start};
 }
+// Tiles of `rows` query rows for many sequences: numbers with gaps, which need no sum over the sequences in front.  Sequence b,
+// whose rows start at `start`, takes those from here to the next sequence's: at least count / rows + `extra` of them.
+FLASH_INDEX uint32_t first_tile(int32_t start, int32_t total, uint32_t rows, uint32_t extra, int32_t b) {
+  return (uint32_t)within(start, 0, total) / rows + extra * (uint32_t)b;
+}
 // keys that row `row` of a sequence with nq queries and nk keys sees
 FLASH_INDEX int32_t visible_keys(int32_t row, int32_t nq, int32_t nk, bool causal) {
   return causal ? within(row + (nk - nq) + 1, 0, nk) : nk;

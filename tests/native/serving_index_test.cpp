@@ -71,6 +71,27 @@ static void prompt_items() {
   }
 }
 
+// the tile numbers of many sequences: in order, room for all of a sequence's tiles (its first one may begin up to 63 rows
+// early where there is room for two more), and all of them inside the grid
+static void tile_numbers() {
+  for (int n = 0; n < 3000; ++n) {
+    const int32_t seqs = 1 + (int32_t)(rnd() % 300);
+    const uint32_t rows = n % 3 == 0 ? 64 : n % 3 == 1 ? 128 : 256, extra = 1 + (uint32_t)(n / 3 % 2);
+    std::vector<int32_t> cu(seqs + 1);
+    cu[0] = (int32_t)(rnd() % 500);
+    for (int b = 0; b < seqs; ++b) cu[b + 1] = cu[b] + (int32_t)(rnd() % (rnd() % 4 ? 20 : 700));
+    const int32_t total = cu[seqs] + (int32_t)(rnd() % 100);
+    const uint32_t grid = (uint32_t)total / rows + extra * (uint32_t)seqs;
+    for (int b = 0; b < seqs; ++b) {
+      const uint32_t shift = extra == 2 ? rnd() % 64 : 0, count = (uint32_t)(cu[b + 1] - cu[b]);
+      const uint32_t mine = count == 0 ? 0 : (count + shift + rows - 1) / rows;
+      const uint32_t first = first_tile(cu[b], total, rows, extra, b), next = first_tile(cu[b + 1], total, rows, extra, b + 1);
+      EXPECT(first + mine <= next && next <= grid);
+    }
+    for (int b = 0; b < seqs; ++b) EXPECT(first_tile(strange(), total, rows, extra, b) < grid + extra);
+  }
+}
+
 static void token_targets() {
   for (int n = 0; n < 20000; ++n) {
     const int32_t seqs = 1 + (int32_t)(rnd() % 9);
@@ -167,6 +188,7 @@ static void the_line() {
 int main() {
   packed_rows();
   prompt_items();
+  tile_numbers();
   token_targets();
   cache_places();
   the_line();

@@ -351,3 +351,15 @@ def test_rows_far_apart(fa, d, dtype, causal):
     kd.copy_(k)
     got = fa.forward_packed(q.cuda(), kd, v.cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda(), causal=causal)
     ref.check_packed(got, q, k, v, q_lens, k_lens, causal, d ** -0.5)
+
+
+@pytest.mark.parametrize("sequences,same,causal,d", [(65, True, True, 128), (64, False, True, 64), (300, False, True, 128), (300, False, False, 64), (4500, True, True, 64)])
+def test_more_sequences_than_a_scan_covers(fa, sequences, same, causal, d):
+    gen = torch.Generator().manual_seed(sequences)
+    q_lens = torch.randint(0, 9, (sequences,), generator=gen).tolist()
+    q_lens[::29] = [200 + b % 70 for b in range(len(q_lens[::29]))]
+    k_lens = q_lens if same else [n + int(x) for n, x in zip(q_lens, torch.randint(-3, 90, (sequences,), generator=gen))]
+    k_lens = [max(0, n) for n in k_lens]
+    q, k, v, _ = make(q_lens, k_lens, 2, 1, d, BF16, seed=25)
+    got = call(fa, q, k, v, q_lens, None if same else k_lens, causal=causal)
+    ref.check_packed(got, q, k, v, q_lens, k_lens, causal, d ** -0.5, heads=[1])
