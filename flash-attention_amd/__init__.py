@@ -251,8 +251,8 @@ def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = T
     query that sees no key gets zeros.  Masked keys and values may hold anything, NaN and infinities included; values
     that are seen are summed in fp32 before they are divided by the weights' sum (bf16 values beyond 1e30 may overflow).
 
-    Returns a new tensor like q, or ``out``; rows behind the last sequence are left as they were.  No backward
-    pass.  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
+    Returns a new tensor like q, or ``out`` (apart from q, k and v in memory); rows behind the last sequence are left as
+    they were.  No backward pass.  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
     return _serving("forward_packed")(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, softmax_scale=softmax_scale,
                                       out=out, sync=sync)
 
