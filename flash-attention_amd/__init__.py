@@ -250,6 +250,7 @@ def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = T
     the keys j <= i + nk - nq: the last query sees the last key, which is what a later piece of a prompt needs.  A
     query that sees no key gets zeros.  Masked keys and values may hold anything, NaN and infinities included; values
     that are seen are summed in fp32 before they are divided by the weights' sum (bf16 values beyond 1e30 may overflow).
+    Scores that are seen are meant to be finite: a query that sees a key with infinite entries may get NaN.
 
     Returns a new tensor like q, or ``out`` (apart from q, k and v in memory); rows behind the last sequence are left as
     they were.  No backward pass.  Blocks until done unless ``sync=False`` (which a graph capture needs)."""

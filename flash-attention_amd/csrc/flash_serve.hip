@@ -33,7 +33,7 @@ int check_heads(int64_t q_heads, int64_t kv_heads, int64_t d) {
   return FLASH_HIP_OK;
 }
 int check_scale(float scale) {
-  REFUSE_IF(!(scale > 0.f) || !std::isfinite(scale), "softmax_scale must be positive and finite (got %g)", (double)scale);
+  REFUSE_IF(!(scale > 0.f) || !std::isfinite(scale * 1.44269504f), "softmax_scale must be positive and finite (got %g)", (double)scale);
   return FLASH_HIP_OK;
 }
 int check_16bit(int dtype) {

@@ -225,7 +225,8 @@ def test_packed_refusals_through_the_abi(fa):
                 vh=64, ot=256, oh=64, softmax_scale=0.125, causal=1, dtype=0)
     for change, match in ((dict(q=None), "null"), (dict(k=None), "null"), (dict(cu_k=None), "cu_seqlens"), (dict(q=P + 4), "16-byte"), (dict(vt=124), "16-byte"),
                           (dict(oh=-64), "negative"), (dict(dtype=2), "float16"), (dict(causal=2), "causal"), (dict(d=52), "head dim"),
-                          (dict(q_heads=5), "multiple"), (dict(total_q=-1), "between"), (dict(total_k=1 << 31), "between"), (dict(softmax_scale=0.0), "softmax_scale")):
+                          (dict(q_heads=5), "multiple"), (dict(total_q=-1), "between"), (dict(total_k=1 << 31), "between"), (dict(softmax_scale=0.0), "softmax_scale"),
+                          (dict(softmax_scale=3e38), "softmax_scale")):
         p = Packed(**{**good, **change})
         assert refused(fa, L.flash_fwd_packed(ctypes.byref(p), None, 0, None), match), change
     # a workspace, where one is of use: few rows over many keys
