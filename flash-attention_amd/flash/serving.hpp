@@ -16,7 +16,8 @@ namespace flash {
 
 // q [total_q, Hq, d], k and v [total_k, Hkv, d], any token and head strides; cu_seqlens_* int32 [sequences + 1].
 // cu_seqlens_k absent: the keys are cut like the queries.  Returns `out`, or a new contiguous tensor like q (rows of
-// no sequence are then undefined).
+// no sequence are then undefined).  Calls with few rows over many keys use scratch (below 70 MB): one buffer for each of
+// torch's streams, one of its own for every captured graph.
 torch::Tensor forward_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                              const torch::Tensor& cu_seqlens_q, const std::optional<torch::Tensor>& cu_seqlens_k,
                              bool causal, std::optional<double> softmax_scale, const std::optional<torch::Tensor>& out,
