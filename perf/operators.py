@@ -11,7 +11,6 @@ import torch
 own = False
 
 DEVICE = "cuda"
-_package = {}
 TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
 E4M3_MAX = 448.0
 #: most work of a drawn case: visible query-key pairs x heads x head dim, scores of the padded batch, cache bytes
@@ -202,10 +201,7 @@ def run(s):
 
 
 def package():
-    """This repository's package, looked up once, as a program that uses it does."""
-    if "module" not in _package:
-        _package["module"] = importlib.import_module("flash-attention_amd")
-    return _package["module"]
+    return importlib.import_module("flash-attention_amd")
 
 
 def softmax_times(scores, visible, v):
