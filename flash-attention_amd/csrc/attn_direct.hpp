@@ -27,6 +27,8 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "serving_index.hpp"
+
 namespace flash_hip {
 namespace direct {
 
@@ -152,11 +154,7 @@ struct Step {
     st.l = 0.f;
   }
 
-  // first of the 8 head-dim elements that lane group g multiplies in k-step ks; a 16-byte load of an 8-bit row holds
-  // those of two k-steps
-  static __device__ __forceinline__ int column(int ks, int g) {
-    return CACHE8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
-  }
+  static __device__ __forceinline__ int column(int ks, int g) { return k_column(CACHE8, ks, g); }
   // element (of a row) where load i of a lane's K begins
   static __device__ __forceinline__ int load_column(int i, int g) { return CACHE8 ? column(2 * i, g) : column(i, g); }
   // key of the step that lane group g multiplies as element j of block s

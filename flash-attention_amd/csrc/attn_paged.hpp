@@ -181,18 +181,21 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
         const char* src = PAGE16 ? kh + tile_start(at, t) : kh + __shfl(at, 16 * t + n);
 #pragma unroll
         for (int i = 0; i < S::kKLoads; ++i) {
-          const int col = S::load_column(i, g);
-          const bool in = FULL || col < p.d;
           if constexpr (PAGE16 && FULL) {
             k[t][i] = stream((const u32x4*)(src + (k_row + (uint32_t)(S::load_column(0, g) * S::kElem)) + S::load_column(i, 0) * S::kElem));
+          } else if constexpr (FULL) {
+            k[t][i] = stream((const u32x4*)(src + (uint32_t)(S::load_column(i, g) * S::kElem)));
           } else {
-            k[t][i] = stream((const u32x4*)(src + ((PAGE16 ? k_row : 0u) + (uint32_t)((in ? col : 0) * S::kElem))));
-          }
-          if constexpr (!FULL) {
-            // (an 8-bit load holds 16 columns, of which the last 8 may lie behind the row)
-            if (!in) k[t][i] = u32x4{0u, 0u, 0u, 0u};
-            if constexpr (CACHE8) {
-              if (in && col + 8 >= p.d) k[t][i][2] = k[t][i][3] = 0u;
+            // (a load never leaves its row: 16 bytes of 8-bit values may be 8 columns more than the row has from there on)
+            constexpr int kWide = 16 / S::kElem;
+            const uint32_t row = PAGE16 ? k_row : 0u;
+            if (kWide > 8 && p.d == 8) {
+              const u32x2 x = stream((const u32x2*)(src + row));
+              k[t][i] = S::load_column(i, g) == 0 ? u32x4{x[0], x[1], 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
+            } else {
+              const RowLoad at_row = row_load(S::load_column(i, g), kWide, p.d);
+              const u32x4 x = stream((const u32x4*)(src + (row + (uint32_t)(at_row.from * S::kElem))));
+              k[t][i] = at_row.skip == 0 ? x : at_row.skip == kWide ? u32x4{0u, 0u, 0u, 0u} : u32x4{x[2], x[3], 0u, 0u};
             }
           }
         }

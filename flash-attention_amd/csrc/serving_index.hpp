@@ -100,6 +100,21 @@ FLASH_INDEX int32_t new_position(const Pages& c, int32_t len, int32_t behind) {
 }
 FLASH_INDEX int32_t cache_length(const Pages& c, int32_t len) { return within(len, 0, c.max_keys); }
 
+// ---- columns of a cache row that a lane loads, of d (a multiple of 8) ------------------------------------------------
+// first of the 8 head-dim elements that lane group g multiplies in k-step ks; a 16-byte load of an 8-bit row holds
+// those of two k-steps
+FLASH_INDEX int32_t k_column(bool cache8, int32_t ks, int32_t g) { return cache8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
+// A load of `width` elements (at most d) where the lane wants those from `column` on: where it begins, inside the row at
+// both ends, and how many elements it skips (`width`: the row has none of them; they count as zeros).
+struct RowLoad {
+  int32_t from, skip;
+};
+FLASH_INDEX RowLoad row_load(int32_t column, int32_t width, int32_t d) {
+  if (column >= d) return RowLoad{0, width};
+  const int32_t from = column + width <= d ? column : d - width;
+  return RowLoad{from, column - from};
+}
+
 // ---- the line of units that decoding workgroups divide among themselves --------------------------------------
 // units of a sequence of n keys; an empty one has a unit too, which writes its zeros
 FLASH_INDEX uint32_t units_of(int32_t n, int32_t unit) { return n <= unit ? 1u : (uint32_t)((n - 1) / unit + 1); }

@@ -1,0 +1,41 @@
+"""GPU: the serving operators at the ends of what they take, against the float64 forms of serving_reference."""
+import pytest
+import torch
+
+import serving_reference as ref
+from test_paged_gpu import check_decode, filled, on_gpu
+
+pytestmark = pytest.mark.gpu
+F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("page,token_major", [(16, False), (4, True)])
+@pytest.mark.parametrize("d", [8, 24, 40, 56, 72, 88, 104, 120, 16, 48, 112])
+def test_rows_at_the_end_of_an_8_bit_cache(fa, d, page, token_major):
+    """Rows that are no whole number of 16-byte loads, the last one of them the cache's last bytes."""
+    lens = [page * 21, page * 3, 5 * page + 1]
+    kc, vc, table, rows = filled(lens, page, 2, d, E4M3, seed=d, token_major=token_major)
+    last = int(table.max())
+    kc, vc = kc[: last + 1], vc[: last + 1]
+    q = torch.randn(3, 6, d, generator=torch.Generator().manual_seed(1)).to(BF16)
+    got, lse = fa.decode_paged(q.cuda(), on_gpu(kc), on_gpu(vc), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softmax_scale=0.003,
+                               return_lse=True)
+    check_decode(got, lse, q, rows, lens, 0.003)
+
+
+def test_last_row_of_a_cache_of_whole_allocation_pages(fa):
+    """80 MiB exactly, of which the last row is read."""
+    page, hk, d, pages = 16, 8, 40, 16384
+    gen = torch.Generator().manual_seed(2)
+    rows = [[torch.randn(48, hk, d, generator=gen).mul(20).to(E4M3)] for _ in range(2)]
+    table = torch.tensor([[pages - 2, 0, pages - 1]], dtype=torch.int32)
+    caches = []
+    for r in rows:
+        c = torch.zeros((pages, hk, page, d), dtype=torch.uint8, device="cuda")
+        assert c.numel() % (2 << 20) == 0
+        for j in range(3):
+            c[int(table[0, j])] = r[0][16 * j:16 * j + 16].view(torch.uint8).transpose(0, 1).cuda()
+        caches.append(c.view(E4M3))
+    q = torch.randn(1, 16, d, generator=gen).to(F16)
+    got = fa.decode_paged(q.cuda(), *caches, table.cuda(), torch.tensor([48], dtype=torch.int32).cuda(), softmax_scale=0.004)
+    check_decode(got, None, q, rows, [48], 0.004)
