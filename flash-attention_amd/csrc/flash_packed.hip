@@ -53,8 +53,9 @@ bool take_half(const packed::Params& p) {
 }
 // The grid's tiles: a sequence has at most two more than whole ones among its rows, its last one and, where its numbers of
 // queries and keys differ and the diagonal is cut, its first one.
-void set_grid(packed::Params& p, int64_t rows) {
-  p.extra = p.causal && !(p.cu_q == p.cu_k && p.total_q == p.total_k) ? 2 : 1;
+int extra_tiles(const packed::Params& p) { return p.causal && !(p.cu_q == p.cu_k && p.total_q == p.total_k) ? 2 : 1; }
+void set_grid(packed::Params& p, int64_t rows, int extra) {
+  p.extra = extra;
   p.tiles = (uint32_t)(p.total_q / rows + (int64_t)p.extra * p.sequences);
   p.items = (uint32_t)packed_grid(p.tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads);
   p.parts = 1;
@@ -63,11 +64,11 @@ void set_grid(packed::Params& p, int64_t rows) {
 // many as fill the chip (two on each of 256 compute units) by what there may be of items.  Measured, cut / whole, us: 128 rows over 32768 keys, 8 heads of 128, 69 / 451; 256 over 8192, 32 heads,
 // 57 / 115; 4096 rows, 4 heads, 41.5 / 60.6; 973 rows of three sequences, 16 heads of 64, 30 / 45; with an item for every
 // compute unit there is nothing to gain: 4096 rows, 8 heads, 64 / 62, 1024 over 8192, 32 heads, 124.6 / 123.
-int parts_of(const packed::Params& p) {
+int parts_of(const packed::Params& p, int extra) {
   constexpr int64_t kUnits = 256, kMostSlots = 4 * kUnits;
   if (!take_half(p) || p.total_k < 2 * m16h::kPartTiles * kBc) return 1;
   packed::Params h = p;
-  set_grid(h, m16h::kPackedRows);
+  set_grid(h, m16h::kPackedRows, extra);
   const int64_t items = ((int64_t)p.total_q / m16h::kPackedRows + p.sequences) * p.heads;
   if (items >= kUnits) return 1;
   const int64_t wanted = (2 * kUnits + items - 1) / items, room = kMostSlots / h.items;
@@ -82,8 +83,8 @@ template <int D, typename TO>
 int launch(packed::Params p, void* workspace, hipStream_t stream) {
   using TH = typename HalfOut<TO>::type;
   if (take_half(p)) {
-    const int parts = workspace ? parts_of(p) : 1;
-    set_grid(p, m16h::kPackedRows);
+    const int extra = extra_tiles(p), parts = workspace ? parts_of(p, extra) : 1;
+    set_grid(p, m16h::kPackedRows, extra);
     if (parts > 1) {
       p.parts = parts;
       p.tickets = (uint32_t*)workspace;
@@ -95,7 +96,7 @@ int launch(packed::Params p, void* workspace, hipStream_t stream) {
     return p.causal ? launch<m16h::attn_fwd_kernel_packed<D, TH, true, false>, m16h::kPackedLds<D>>(p, stream)
                     : launch<m16h::attn_fwd_kernel_packed<D, TH, false, false>, m16h::kPackedLds<D>>(p, stream);
   }
-  set_grid(p, m16::kPackedRows);
+  set_grid(p, m16::kPackedRows, extra_tiles(p));
   return p.causal ? launch<m16::attn_fwd_kernel_packed<D, TO, true, false>, m16::kPackedLds<D>>(p, stream)
                   : launch<m16::attn_fwd_kernel_packed<D, TO, false, false>, m16::kPackedLds<D>>(p, stream);
 }
@@ -109,12 +110,19 @@ bool packed_mfma_takes(const packed::Params& p) {
          packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads) < (1ull << 31);
 }
 
+// By sizes alone: room for the call whether its keys are cut like its queries (the same offsets, known at the launch) or not.
 int64_t packed_mfma_workspace(const packed::Params& p) {
-  const int parts = packed_mfma_takes(p) ? parts_of(p) : 1;
-  if (parts == 1) return 0;
-  packed::Params h = p;
-  set_grid(h, m16h::kPackedRows);
-  return FLASH_PACKED_TICKET_BYTES + (int64_t)h.items * parts * part_floats(p) * 4;
+  if (!packed_mfma_takes(p)) return 0;
+  int64_t most = 0;
+  for (int extra = p.causal && p.total_q != p.total_k ? 2 : 1; extra <= (p.causal ? 2 : 1); ++extra) {
+    const int parts = parts_of(p, extra);
+    if (parts == 1) continue;
+    packed::Params h = p;
+    set_grid(h, m16h::kPackedRows, extra);
+    const int64_t bytes = FLASH_PACKED_TICKET_BYTES + (int64_t)h.items * parts * part_floats(p) * 4;
+    most = bytes > most ? bytes : most;
+  }
+  return most;
 }
 
 int launch_packed_mfma(const packed::Params& p, bool bf16, void* workspace, hipStream_t stream) {

@@ -39,3 +39,18 @@ def test_last_row_of_a_cache_of_whole_allocation_pages(fa):
     q = torch.randn(1, 16, d, generator=gen).to(F16)
     got = fa.decode_paged(q.cuda(), *caches, table.cuda(), torch.tensor([48], dtype=torch.int32).cuda(), softmax_scale=0.004)
     check_decode(got, None, q, rows, [48], 0.004)
+
+
+@pytest.mark.parametrize("heads,lens", [(8, [1700]), (8, [1000, 2000]), (2, [2048]), (16, [1536])])
+def test_as_many_keys_as_queries_with_offsets_of_their_own(fa, heads, lens):
+    """Key offsets in a tensor of their own, with the same totals: the same result as without, and other places too."""
+    gen = torch.Generator().manual_seed(heads)
+    total, d = sum(lens), 64
+    q, k, v = (torch.randn(total, h, d, generator=gen).to(F16) for h in (heads, 1, 1))
+    cu = ref.offsets(lens).cuda()
+    args = [x.cuda() for x in (q, k, v)]
+    got = fa.forward_packed(*args, cu, cu.clone())
+    ref.check_packed(got, q, k, v, lens, lens, True, d ** -0.5, heads=[0, heads - 1])
+    k_lens = [lens[0] + 0] if len(lens) == 1 else [lens[0] + 300, lens[1] - 300]
+    got = fa.forward_packed(*args, cu, ref.offsets(k_lens).cuda())
+    ref.check_packed(got, q, k, v, lens, k_lens, True, d ** -0.5, heads=[0, heads - 1])
