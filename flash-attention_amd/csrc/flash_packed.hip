@@ -103,11 +103,13 @@ int launch(packed::Params p, void* workspace, hipStream_t stream) {
 
 }  // namespace
 
+// (the grids of cut items have at most 1024 workgroups, see parts_of)
+static_assert(m16::kThreads == m16h::kThreads, "one limit of the grid");
 bool packed_mfma_takes(const packed::Params& p) {
   const int64_t most = (int64_t)kOob / m16::kPackedRows;  // a row's bytes: 256 of them stay below kOob
   const int64_t tiles = (int64_t)p.total_q / m16h::kPackedRows + 2 * (int64_t)p.sequences;
   return p.q_token <= most && p.o_token <= most && p.k_token <= most && p.v_token <= most && tiles < ((int64_t)1 << 31) &&
-         packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads) < (1ull << 31);
+         grid_fits(packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads), m16::kThreads);
 }
 
 // By sizes alone: room for the call whether its keys are cut like its queries (the same offsets, known at the launch) or not.

@@ -148,11 +148,12 @@ int launch_decode(const DecodeParams& p, int dtype, bool cache8, hipStream_t str
 }
 
 // ---- packed prompts -----------------------------------------------------------------------------------------------
+int64_t direct_tiles(const flash_hip::packed::Params& p) { return (int64_t)p.total_q / flash_hip::packed::kDirectRows + p.sequences; }
 template <int D, int EK>
 int launch_packed_direct(flash_hip::packed::Params p, hipStream_t stream) {
   namespace pk = flash_hip::packed;
   p.extra = 1;
-  p.tiles = (uint32_t)(p.total_q / pk::kDirectRows + p.sequences);
+  p.tiles = (uint32_t)direct_tiles(p);
   const dim3 grid(p.tiles, (uint32_t)p.heads);
   if (p.d == D) {
     hipLaunchKernelGGL((pk::packed_direct_kernel<D, EK, true>), grid, dim3(256), 0, stream, p);
@@ -202,6 +203,9 @@ int plan_packed(const flash_packed_args* a, bool memory, flash_hip::packed::Para
   p.d = (int32_t)a->d;
   p.causal = a->causal;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  // (many short sequences times heads pass the pipelined kernel's grid first; the other one has the heads in a dimension of their own)
+  REFUSE_IF(!flash_hip::packed_mfma_takes(p) && !flash_hip::grid_fits((uint64_t)direct_tiles(p), 256),
+            "%lld sequences of %lld rows in all are too many for one call", (long long)a->sequences, (long long)a->total_q);
   return FLASH_HIP_OK;
 }
 
@@ -259,7 +263,8 @@ int flash_cache_append(const flash_append_args* a, const flash_paged_cache* c, v
   REFUSE_IF(!a, "null flash_append_args");
   CHECK(check_cache(c, a->dtype, true));
   CHECK(check_heads(c->kv_heads, c->kv_heads, c->d));
-  REFUSE_IF(a->tokens < 0 || a->tokens > kMostIndex, "between 0 and 2^30 tokens (got %lld)", (long long)a->tokens);
+  REFUSE_IF(a->tokens < 0 || !flash_hip::grid_fits((uint64_t)a->tokens / ap::kMostTokens + 1, ap::kThreads),
+            "between 0 and %lld tokens (got %lld)", (1ll << 32) / ap::kThreads * ap::kMostTokens - ap::kMostTokens - 1, (long long)a->tokens);
   REFUSE_IF(!a->cu_seqlens && a->tokens != c->sequences, "without cu_seqlens one token per sequence is needed (got %lld tokens, %lld sequences)",
             (long long)a->tokens, (long long)c->sequences);
   if (a->tokens == 0 || c->sequences == 0) return FLASH_HIP_OK;

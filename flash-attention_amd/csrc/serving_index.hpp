@@ -15,6 +15,9 @@ namespace flash_hip {
 
 FLASH_INDEX int32_t within(int32_t x, int32_t low, int32_t high) { return x < low ? low : (x > high ? high : x); }
 
+// Workgroups that one dimension of a grid can have: the runtime refuses 2^32 threads and more along it
+FLASH_INDEX bool grid_fits(uint64_t workgroups, uint32_t threads) { return workgroups < (1ull << 32) / threads; }
+
 // ---- packed sequences -------------------------------------------------------------------------------------------
 struct Range {
   int32_t start, count;

@@ -245,7 +245,8 @@ typedef enum flash_hip_dtype { FLASH_F16 = 0, FLASH_BF16 = 1, FLASH_E4M3 = 2 } f
  * Attention over packed prompts.  Sequence b = 0 .. sequences - 1 has the queries cu_seqlens_q[b] ..
  * cu_seqlens_q[b + 1] - 1 of q and the keys cu_seqlens_k[b] .. cu_seqlens_k[b + 1] - 1 of k and v; with `causal` its
  * query i sees key j when j <= i + (its keys - its queries): the last query sees the last key.  A query that sees
- * no key gets zeros.  Rows of o that belong to no sequence are left as they were.
+ * no key gets zeros.  Rows of o that belong to no sequence are left as they were.  (Calls with 2^24 or more of
+ * sequences + total_q / 64 may be refused: a launch does not take them.)
  */
 typedef struct flash_packed_args {
   const void* q;                 /* [total_q, q_heads, d] */
@@ -322,7 +323,7 @@ int64_t flash_decode_paged_workspace_bytes(const flash_decode_args* args, const 
  * cu_seqlens[b + 1] - 1 belong to sequence b (cu_seqlens NULL: row b, tokens == sequences) and take its last
  * positions, seq_lens[b] counting them already.  Into an e4m3 cache goes the nearest value to x / scale, ties to
  * even, the largest for what lies beyond it.  Rows of no sequence, positions outside the table and pages outside the
- * cache are not written; two rows for one position leave either.
+ * cache are not written; two rows for one position leave either.  Fewer than 2^29 - 32 tokens a call.
  */
 typedef struct flash_append_args {
   const void* k;

@@ -1,5 +1,6 @@
 // Host walk through the loads of decoding's cache rows (csrc/serving_index.hpp): for every head dim, tile and width of a
-// cache element no load of K or V leaves its row at either end, and every column is multiplied once.
+// cache element no load of K or V leaves its row at either end, and every column is multiplied once.  And through the
+// rule for grids that the runtime takes.
 #include <cstdio>
 #include <cstdlib>
 #include <vector>
@@ -45,6 +46,11 @@ int main() {
         EXPECT(from + mine <= d);
       }
     }
+  }
+  for (int threads : {64, 256, 1024}) {
+    const int d = threads;
+    EXPECT(grid_fits(1, threads) && !grid_fits((1ull << 32) / threads, threads) && !grid_fits(1ull << 63, threads));
+    EXPECT(grid_fits((1ull << 32) / threads - 1, threads) && ((1ull << 32) / threads - 1) * threads < 1ull << 32);
   }
   printf("loads stay inside their rows\n");
   return 0;

@@ -54,3 +54,24 @@ def test_as_many_keys_as_queries_with_offsets_of_their_own(fa, heads, lens):
     k_lens = [lens[0] + 0] if len(lens) == 1 else [lens[0] + 300, lens[1] - 300]
     got = fa.forward_packed(*args, cu, ref.offsets(k_lens).cuda())
     ref.check_packed(got, q, k, v, lens, k_lens, True, d ** -0.5, heads=[0, heads - 1])
+
+
+def test_more_short_prompts_than_one_dimension_of_a_grid_holds(fa):
+    """2^19 prompts of a row or two, 32 heads: over 2^24 (prompt, head) pairs."""
+    heads, d, sequences = 32, 8, 1 << 19
+    lens = torch.ones(sequences, dtype=torch.int64)
+    lens[5::1000] = 0
+    lens[7::997] = 2
+    lens[:4] = torch.tensor([70, 3, 0, 130])
+    total = int(lens.sum())
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(total, heads, d, generator=gen, device="cuda").to(BF16)
+    k, v = (torch.randn(total, 1, d, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
+    got = fa.forward_packed(q, k, v, cu.to(torch.int32).cuda())
+    ref.check_packed(got[:203], q[:203], k[:203], v[:203], [70, 3, 0, 130], [70, 3, 0, 130], True, d ** -0.5, heads=[0, 31])
+    first = cu[:-1][lens > 0].cuda()            # a prompt's first row sees itself alone
+    assert torch.equal(got[first], v[first].expand(-1, heads, -1))
+    last = total - int(lens[-600:].sum())
+    tail = [int(n) for n in lens[-600:]]
+    ref.check_packed(got[last:], q[last:], k[last:], v[last:], tail, tail, True, d ** -0.5, heads=[17])

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import ROOT
-from test_serving_host import P, Packed, refused
+from test_serving_host import P, Append, Packed, cache, refused
 
 F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
 
@@ -40,3 +40,23 @@ def test_scratch_of_packed_prompts_follows_from_sizes(fa, q_heads, causal):
                 assert refused(fa, L.flash_fwd_packed(ctypes.byref(call), P + 8, need, None), "aligned")
                 if need > 0:
                     assert refused(fa, L.flash_fwd_packed(ctypes.byref(call), P + 8, need - 1, None), "too small")
+
+
+def test_grids_that_no_launch_takes_are_refused(fa):
+    """2^24 workgroups of 256 threads and more along one dimension."""
+    L = fa.lib()
+    a = dict(q=P, k=P, v=P, o=P, cu_q=P, cu_k=P, total_q=6, total_k=6, q_heads=4, kv_heads=2, d=64, qt=256, qh=64, kt=128, kh=64, vt=128,
+             vh=64, ot=256, oh=64, softmax_scale=0.125, causal=1, dtype=0)
+    for sequences in (1 << 24, 1 << 30):
+        assert refused(fa, L.flash_fwd_packed(ctypes.byref(Packed(**a, sequences=sequences)), None, 0, None), "too many")
+        assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(Packed(**a, sequences=sequences))) == -1
+    for sequences, heads in ((1 << 20, 64), ((1 << 24) - 1, 4), (1, 4)):      # heads have a dimension of their own
+        call = Packed(**{**a, "sequences": sequences, "q_heads": heads, "qt": heads * 64, "ot": heads * 64})
+        assert L.flash_fwd_packed_workspace_bytes(ctypes.byref(call)) == 0
+        assert refused(fa, L.flash_fwd_packed(ctypes.byref(call), P + 8, 0, None), "aligned")
+    one_row = dict(k=P, v=P, k_token_stride=128, k_head_stride=64, v_token_stride=128, v_head_stride=64, cu_seqlens=P, dtype=0)
+    for tokens in ((1 << 29) - 32, 1 << 29, 1 << 30):
+        x = Append(**one_row, tokens=tokens)
+        assert refused(fa, L.flash_cache_append(ctypes.byref(x), ctypes.byref(cache()), None), "tokens")
+    x = Append(**{**one_row, "k": P + 8}, tokens=(1 << 29) - 33)
+    assert refused(fa, L.flash_cache_append(ctypes.byref(x), ctypes.byref(cache()), None), "16-byte")
