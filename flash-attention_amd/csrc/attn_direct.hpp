@@ -20,6 +20,9 @@
 // Where K and V come from memory for one use (decoding), P is kept as a sum of two 16-bit values, p = hi + lo with
 // |lo| <= 2^-8 p (bf16) or 2^-11 p (fp16), and both are multiplied: the second product costs matrix cycles that a kernel
 // bound by memory has to spare, and the result carries the rounding of the output alone.  For prompts P is rounded once.
+// fp16 has no bits below 2^-24, and a long tail behind one leading key consists of small weights: they are raised by 2^15
+// (the largest, 1, stays below 65504) before they are rounded, which keeps them down to 2^-39 of the largest.  The sums of
+// products carry that factor until they are divided by l, which does not.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -45,6 +48,8 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 constexpr int kHalf = 0;      // IEEE binary16 operands
 constexpr int kBfloat = 1;    // bfloat16 operands
 constexpr float kMinusInf = -__builtin_huge_valf();
+template <int EK>
+constexpr float kRaise = EK == kHalf ? 32768.f : 1.f;  // of the weights in the second product
 
 // N 32-bit words, as loaded
 template <int N>
@@ -197,7 +202,7 @@ struct Step {
   // (wave-uniform).  LIMIT: the lane's query sees the first `limit` keys of the step only (fewer than one: none).
   struct Weights {
     u32x4 hi[NS], lo[NS];
-    float p[2 * NS][4];  // as computed (LIMIT only)
+    float p[2 * NS][4];  // before they were rounded (LIMIT only)
   };
   template <bool LIMIT>
   static __device__ __forceinline__ void weigh(State& st, Weights& w, const KBlock& k, const u32x4 (&qf)[kKS], uint64_t valid, float c,
@@ -258,6 +263,7 @@ struct Step {
       for (int i = 0; i < 4; ++i) {
         s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
         sum += s[t][i];
+        s[t][i] *= kRaise<EK>;
         if constexpr (LIMIT) w.p[t][i] = s[t][i];
       }
     }

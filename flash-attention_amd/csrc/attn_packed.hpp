@@ -156,7 +156,7 @@ __device__ __forceinline__ void attend_rows(const Params& p, const Tile& t, int3
     S::accumulate_limited(st, w, v, lane, sees - key0);
   }
   const float l = quad_sum(st.l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / kRaise<EK> / l;
   if (!mine) return;
   char* dst = p.o + (int64_t)(t.q0 + row) * p.o_token + (int64_t)head * p.o_head;
 #pragma unroll

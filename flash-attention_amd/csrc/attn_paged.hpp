@@ -244,7 +244,7 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     // ---- the four waves' parts --------------------------------------------------------------------------
     const bool complete = u0 == 0 && u1 == units;
     const uint32_t slot = part_slot(blockIdx.x, c, r - u0);
-    const float vs = CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f;
+    const float vs = (CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f) * (1.f / kRaise<EK>);  // and what the weights are raised by
     const float l = quad_sum(st.l);
     if (g == 0) {
       sh_ml[wave][n][0] = st.m;

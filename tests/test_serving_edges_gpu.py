@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import serving_bounds as bounds
 import serving_reference as ref
 from test_paged_gpu import check_decode, filled, on_gpu
 
@@ -75,3 +76,43 @@ def test_more_short_prompts_than_one_dimension_of_a_grid_holds(fa):
     last = total - int(lens[-600:].sum())
     tail = [int(n) for n in lens[-600:]]
     ref.check_packed(got[last:], q[last:], k[last:], v[last:], tail, tail, True, d ** -0.5, heads=[17])
+
+
+def leading_key(n, heads, d, at, ahead, dtype, seed, tail=1.0):
+    """(k, v): scores of about 0 against a query of ones at scale 1 / d, but for key `at`, which leads by `ahead` powers of
+    two and has the value 0 (a key that takes what attention is not needed elsewhere); the others' values have mean `tail`."""
+    gen = torch.Generator().manual_seed(seed)
+    k = torch.randn(n, heads, d, generator=gen) * 0.05
+    k[at] = ahead * 0.6931
+    v = tail + 0.25 * torch.randn(n, heads, d, generator=gen)
+    v[at] = 0.0
+    return k.to(dtype), v.to(dtype)
+
+
+@pytest.mark.parametrize("ahead", [4, 14, 20, 24, 27, 31, 36])
+@pytest.mark.parametrize("n,page,d,dtype,cache", [(20011, 16, 128, F16, F16), (300, 16, 64, F16, F16), (4000, 8, 72, F16, F16), (20011, 16, 64, BF16, BF16),
+                                                  (5000, 32, 128, F16, E4M3)])
+def test_decoding_with_one_leading_key(fa, n, page, d, dtype, cache, ahead):
+    """The tail's weights, far below the leading one's, are what the result consists of."""
+    ks, vs = (torch.tensor([0.0625]), torch.tensor([0.25])) if cache == E4M3 else (None, None)
+    k, v = leading_key(n, 1, d, n // 3, ahead, torch.float32, 7)
+    rows = [[(x if s is None else x / s).to(cache)] for x, s in ((k, ks), (v, vs))]
+    kc, vc, table = ref.page_pool([n], page, 1, d, cache, seed=3)
+    for c, r in zip((kc, vc), rows):
+        ref.fill(c, table, r, page)
+    q = torch.ones(1, 2, d, dtype=dtype)
+    dev = [None if s is None else s.cuda() for s in (ks, vs)]
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), softmax_scale=1.0 / d,
+                          k_scale=dev[0], v_scale=dev[1])
+    bounds.check_decoding(got, q, rows, [n], 1.0 / d, ks, vs, what=f"{ahead} ahead")
+
+
+@pytest.mark.parametrize("cut", [0, 1])
+@pytest.mark.parametrize("d,dtype,cache", [(128, F16, F16), (64, BF16, BF16), (112, BF16, E4M3)])
+def test_decoding_within_the_bounds_of_its_weights(fa, d, dtype, cache, cut):
+    lens = [[700, 33, 1], [9000]][cut]
+    kc, vc, table, rows = filled(lens, 16, 2, d, cache, seed=d)
+    q = torch.randn(len(lens), 4, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+    scale = 0.01 if cache == E4M3 else d ** -0.5
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softmax_scale=scale)
+    bounds.check_decoding(got, q, rows, lens, scale)
