@@ -624,10 +624,12 @@ __device__ __forceinline__ void forget_max(float& mx_all) {
 
 // OWN_ROWS: only queries whose own maximum passed the threshold move their reference, so that a query's result does not
 // depend on the other queries of its wave (otherwise all queries of the wave move theirs, up, to where they stand).
+// `lift`: how far below its queries' maximum a reference that moves comes to stand, as a part of the threshold.
 template <int NB, bool HAS_NEXT, bool PIN = false, bool OWN_ROWS = false>
 __device__ __forceinline__ void step_end(f32x4 (&o)[kQ16][NB], State (&st)[kQ16], const float mx_all,
                                          f32x4 (&lsum)[kQ16], f32x4 (&bias)[kQ16], f32x4 (&s_nxt)[2][kQ16],
-                                         uint64_t& pending, const uint64_t vote, const ScaleSplit sc, int lane) {
+                                         uint64_t& pending, const uint64_t vote, const ScaleSplit sc, int lane,
+                                         const float lift = 0.f) {
   // `vote` = pending-rescale mask | lanes whose next-block maximum exceeds the threshold (pipeline_step)
   if constexpr (PIN) pin_tiles(s_nxt, bias);
   if (__builtin_expect(vote != 0, 0)) {
@@ -658,7 +660,7 @@ __device__ __forceinline__ void step_end(f32x4 (&o)[kQ16][NB], State (&st)[kQ16]
         const float mq = fmaxf(fmaxf(fmaxf(t0[0], t0[1]), fmaxf(t0[2], t0[3])),
                                fmaxf(fmaxf(t1[0], t1[1]), fmaxf(t1[2], t1[3])));
         const float top = quad_lane_max(mq, lane);
-        const float rise = OWN_ROWS ? (top > sc.thr ? top : 0.f) : fmaxf(top, 0.f);  // references only move up
+        const float rise = OWN_ROWS ? (top > sc.thr ? top - lift * sc.thr : 0.f) : fmaxf(top, 0.f);  // references only move up
         st[q].alpha = fast_exp2(-rise * sc.c);
         st[q].mc += rise;
 #pragma unroll

@@ -15,6 +15,16 @@ constexpr int kPeriod = kVBlocks == 4 ? 6 : 3;  // tiles after which both rings 
 template <int D>
 constexpr int kPackedLds = kRing * Cfg<D>::kTileBytes + kVBlocks * Cfg<D>::kBlkBytes;
 
+// How far (in exp2 units) a row's largest weight stands above 1 when its reference moves.  fp16 has no bits below 2^-24, and
+// a long tail behind one leading key consists of small weights: they are raised by 2^7, which with the 2^8 that the
+// reference may lag behind stays below 65504 and keeps weights down to 2^-31 of the largest.  (bfloat16 reaches as
+// far down as fp32.)  Where |reference| is so large that fp32 has no room for the lift, rounding makes it up to twice
+// as much or nothing: below 2^15 all the same.
+template <int EK>
+constexpr float kLift = EK == kF16 ? 7.f : 0.f;
+template <int EK>
+constexpr float kLiftOfThreshold = kLift<EK> / (kDeferLog2 + kLift<EK>);
+
 // A tile iteration: tile t with (t + lead) % kPeriod = SLOT.  Q0 is the first query block that sees tile t, QK_B the first
 // one that sees tile t + 1, PV_A the first one that saw tile t - 1; MASK_A and MASK_B the block whose scores of tile t
 // (second half) and tile t + 1 (first half) are masked; QK_NEXT: there is a tile t + 1, STAGE_K: a tile t + 2.
@@ -115,7 +125,8 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
   // which may be partly there
   const int full = SPLIT ? part.behind - part.first - (CAUSAL ? kQ16 : 1) : (CAUSAL ? a0 / kBc : (it.nk - 1) / kBc);
   const int lead = (kPeriod - full % kPeriod) % kPeriod;
-  const ScaleSplit sc{p.scale_log2, kDeferLog2 / p.scale_log2};
+  // (finite: a scale below 1e-37 must not make the lift infinite)
+  const ScaleSplit sc{p.scale_log2, fminf((kDeferLog2 + kLift<EK>) / p.scale_log2, 3e38f)};
 
   const char* const qb = p.q + ((int64_t)it.q0 + row0) * p.q_token + (int64_t)head * p.q_head;
   char* const ob = p.o + ((int64_t)it.q0 + row0) * p.o_token + (int64_t)head * p.o_head;
@@ -261,7 +272,7 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
     mask_tile(sA[1][q], 16, key_limit(limit, q), lane);
     float mx = fmaxf(fmaxf(sA[0][q][0], sA[0][q][1]), fmaxf(sA[0][q][2], sA[0][q][3]));
     mx = fmaxf(mx, fmaxf(fmaxf(sA[1][q][0], sA[1][q][1]), fmaxf(sA[1][q][2], sA[1][q][3])));
-    const float mc = quad_lane_max(mx, lane);  // every row sees key 0
+    const float mc = quad_lane_max(mx, lane) - kLiftOfThreshold<EK> * sc.thr;  // every row sees key 0
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sA[0][q][i] -= mc;
@@ -304,10 +315,10 @@ __device__ __forceinline__ bool packed_item(const packed::Params& p, packed::Ite
     pipeline_step<D, true, F::QK_NEXT, F::MASK_A != kNoMask, kPvAccumulate, EK, true, F::Q0, F::Q0, F::PV_A, (F::MASK_A < 0 ? -1 : F::MASK_A)>(
         hook1, k_cur + kBlkBytes, v_prv, k_nxt, la, bias, qf, ka, o, sA, sB, pB, pA, mx_all, lsum, sc, pending, vote, t * kBc + 32,
         limit, lane);
-    step_end<kDv16, true, false, true>(o, st, mx_all, lsum, bias, sB, pending, vote, sc, lane);
+    step_end<kDv16, true, false, true>(o, st, mx_all, lsum, bias, sB, pending, vote, sc, lane, kLiftOfThreshold<EK>);
     pipeline_step<D, F::QK_NEXT, F::QK_NEXT, F::MASK_B != kNoMask, kPvAccumulate, EK, true, F::QK_B, F::Q0, F::Q0, (F::MASK_B < 0 ? -1 : F::MASK_B)>(
         hook2, k_nxt, v_cur, k_nxt + kBlkBytes, la, bias, qf, ka, o, sB, sA, pA, pB, mx_all, lsum, sc, pending, vote, (t + 1) * kBc, limit, lane);
-    step_end<kDv16, F::QK_NEXT, false, true>(o, st, mx_all, lsum, bias, sA, pending, vote, sc, lane);
+    step_end<kDv16, F::QK_NEXT, false, true>(o, st, mx_all, lsum, bias, sA, pending, vote, sc, lane, kLiftOfThreshold<EK>);
     staged_barrier();
   };
   constexpr int kEndMask = CAUSAL ? 0 : kMaskAll;  // of the end's first tile (idle in front of the other tiles)

@@ -116,3 +116,54 @@ def test_decoding_within_the_bounds_of_its_weights(fa, d, dtype, cache, cut):
     scale = 0.01 if cache == E4M3 else d ** -0.5
     got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softmax_scale=scale)
     bounds.check_decoding(got, q, rows, lens, scale)
+
+
+PROMPTS = [
+    # q_lens, k_lens, query heads, d, type, causal, K rows apart (0: adjacent)
+    ([400, 90], [400, 90], 2, 128, F16, True, 0),           # 128-row items
+    ([300], [700], 2, 64, F16, False, 0),
+    ([4200], [4200], 32, 64, F16, True, 0),                 # 256-row items
+    ([70], [6000], 2, 128, F16, True, 0),                   # the keys of a row dealt to several workgroups
+    ([33, 150], [2500, 3100], 2, 72, F16, False, 0),
+    ([60], [300], 2, 64, F16, True, (1 << 21) + 64),        # row by row
+    ([400], [400], 2, 64, BF16, True, 0),
+    ([70], [6000], 2, 128, BF16, True, 0),
+]
+
+
+@pytest.mark.parametrize("at,ahead", [(0, 4), (0, 20), (0, 25), (0, 29), (0.4, 14), (0.4, 20), (0.4, 25), (0.9, 25), ("two", 14), ("two", 18)])
+@pytest.mark.parametrize("case", PROMPTS, ids=lambda c: f"q{'-'.join(map(str, c[0]))}_k{'-'.join(map(str, c[1]))}_{c[2]}h_d{c[3]}_{str(c[4])[6:]}_{'causal' if c[5] else 'all'}_{c[6]}")
+def test_prompts_with_one_leading_key(fa, case, at, ahead):
+    """As for decoding.  "two": the first key leads and one in the middle leads by 7.5 powers of two more, which moves no
+    reference."""
+    q_lens, k_lens, heads, d, dtype, causal, apart = case
+    parts = []
+    for b, n in enumerate(k_lens):
+        k, v = leading_key(n, 1, d, 0 if at == "two" else int(at * n), ahead, dtype, b)
+        if at == "two":
+            k[n // 2], v[n // 2] = ((ahead + 7.5) * 0.6931), 0.0
+        parts.append((k, v))
+    k, v = (torch.cat(x) for x in zip(*parts))
+    q = torch.ones(sum(q_lens), heads, d, dtype=dtype)
+    kd = k.cuda()
+    if apart:
+        kd = torch.zeros(k.shape[0], apart, dtype=dtype, device="cuda")[:, :d].unflatten(1, (1, d))
+        kd.copy_(k)
+    got = fa.forward_packed(q.cuda(), kd, v.cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda(), causal=causal, softmax_scale=1.0 / d)
+    bounds.check_prompts(got, q, k, v, q_lens, k_lens, causal, 1.0 / d, heads=[0])
+
+
+@pytest.mark.parametrize("case", PROMPTS, ids=lambda c: f"q{'-'.join(map(str, c[0]))}_k{'-'.join(map(str, c[1]))}_{c[2]}h_d{c[3]}_{str(c[4])[6:]}_{'causal' if c[5] else 'all'}_{c[6]}")
+@pytest.mark.parametrize("scale", [0.125, 2.0, 1e-30, 2e-38])
+def test_prompts_within_the_bounds_of_their_weights(fa, case, scale):
+    """Ordinary values, at ordinary scales and where the softmax has one key or all of them."""
+    q_lens, k_lens, heads, d, dtype, causal, apart = case
+    gen = torch.Generator().manual_seed(sum(k_lens))
+    q = torch.randn(sum(q_lens), heads, d, generator=gen).to(dtype)
+    k, v = (torch.randn(sum(k_lens), 1, d, generator=gen).to(dtype) for _ in range(2))
+    kd = k.cuda()
+    if apart:
+        kd = torch.zeros(k.shape[0], apart, dtype=dtype, device="cuda")[:, :d].unflatten(1, (1, d))
+        kd.copy_(k)
+    got = fa.forward_packed(q.cuda(), kd, v.cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda(), causal=causal, softmax_scale=scale)
+    bounds.check_prompts(got, q, k, v, q_lens, k_lens, causal, scale, heads=[0])
