@@ -21,8 +21,10 @@
 // |lo| <= 2^-8 p (bf16) or 2^-11 p (fp16), and both are multiplied: the second product costs matrix cycles that a kernel
 // bound by memory has to spare, and the result carries the rounding of the output alone.  For prompts P is rounded once.
 // fp16 has no bits below 2^-24, and a long tail behind one leading key consists of small weights: they are raised by 2^15
-// (the largest, 1, stays below 65504) before they are rounded, which keeps them down to 2^-39 of the largest.  The sums of
-// products carry that factor until they are divided by l, which does not.
+// (the largest, 1, stays below 65504) before they are rounded, which keeps them down to 2^-39 of the largest.  bfloat16
+// reaches as far as fp32, and the sum of a few values near its end does not fit fp32: its weights are lowered by 2^31,
+// one for each of the 2^30 positions that there may be.  The sums of products carry that factor until they are divided by
+// l, which does not.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -49,7 +51,7 @@ constexpr int kHalf = 0;      // IEEE binary16 operands
 constexpr int kBfloat = 1;    // bfloat16 operands
 constexpr float kMinusInf = -__builtin_huge_valf();
 template <int EK>
-constexpr float kRaise = EK == kHalf ? 32768.f : 1.f;  // of the weights in the second product
+constexpr float kRaise = EK == kHalf ? 0x1p15f : 0x1p-31f;  // of the weights in the second product
 
 // N 32-bit words, as loaded
 template <int N>

@@ -167,3 +167,19 @@ def test_prompts_within_the_bounds_of_their_weights(fa, case, scale):
         kd.copy_(k)
     got = fa.forward_packed(q.cuda(), kd, v.cuda(), ref.offsets(q_lens).cuda(), ref.offsets(k_lens).cuda(), causal=causal, softmax_scale=scale)
     bounds.check_prompts(got, q, k, v, q_lens, k_lens, causal, scale, heads=[0])
+
+
+@pytest.mark.parametrize("page,lens", [(16, [2, 700, 3000]), (2, [40]), (16, [20000])])
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 40), (F16, 64)])
+def test_decoding_values_at_the_end_of_the_range(fa, page, lens, dtype, d):
+    """Means of the type's largest values are finite, whatever their sum would be."""
+    kc, vc, table, rows = filled(lens, page, 1, d, dtype, seed=5)
+    gen = torch.Generator().manual_seed(4)
+    rows[1] = [(torch.finfo(dtype).max * (0.5 + 0.49 * torch.rand(n, 1, d, generator=gen))).to(dtype) for n in lens]
+    for b in range(len(lens)):
+        rows[1][b][:, :, ::3] *= -1
+        rows[1][b][1::2, :, 1::3] *= -1
+    ref.fill(vc, table, rows[1], page)
+    q = torch.randn(len(lens), 2, d, generator=gen).to(dtype)
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    bounds.check_decoding(got, q, rows, lens, d ** -0.5)
