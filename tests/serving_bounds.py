@@ -55,8 +55,9 @@ class Head:
         relative = 2 * ((self.d + 8) * 2.0 ** -24 * (self.rise + 1) + 2 * 2.0 ** -23) + 2 * (self.keys / 8 + 40) * 2.0 ** -24
         weights = u * (self.spread + self.out.abs()) if single else 2 * u * u * self.spread
         floor = SMALLEST[dtype] / top * self.top
-        lost = torch.minimum(self.p, floor) @ self.v.abs()
-        return u * self.out.abs() + SMALLEST[dtype] + (1 + u) * (weights + relative * self.spread + 2 * lost) + 1e-38
+        least = torch.minimum(self.p, floor)
+        lost = least @ self.v.abs() + least.sum(1, keepdim=True) * self.out.abs()
+        return u * self.out.abs() + SMALLEST[dtype] + (1 + u) * (weights + relative * self.spread + lost) + 1e-38
 
     def may_overflow(self):
         """Where a prompt's sum of products, before it is divided, may pass the range of fp32 (half of it: the sum's own

@@ -183,3 +183,33 @@ def test_decoding_values_at_the_end_of_the_range(fa, page, lens, dtype, d):
     q = torch.randn(len(lens), 2, d, generator=gen).to(dtype)
     got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
     bounds.check_decoding(got, q, rows, lens, d ** -0.5)
+
+
+@pytest.mark.parametrize("nq,nk,d,dtype,causal", [(333, 333, 128, BF16, True), (290, 290, 64, F16, True), (150, 2300, 128, BF16, True), (90, 400, 72, BF16, False),
+                                                 (60, 300, 64, F16, False)])
+def test_prompts_with_the_lowest_values(fa, nq, nk, d, dtype, causal):
+    """The type's lowest value in some values, seen by some rows and not by others: within the ordinary bound, or, where the
+    sum of the products may pass the range of fp32, an infinity of the right sign; never another number, never NaN."""
+    gen = torch.Generator().manual_seed(nk)
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(dtype) for n, h in ((nq, 2), (nk, 1), (nk, 1)))
+    for row in (40, nk - 149, nk - 70, nk - 3):
+        v[max(row, 0), 0, 3::7] = torch.finfo(dtype).min
+    got = fa.forward_packed(q.cuda(), k.cuda(), v.cuda(), ref.offsets([nq]).cuda(), ref.offsets([nk]).cuda(), causal=causal)
+    bounds.check_prompts(got, q, k, v, [nq], [nk], causal, d ** -0.5)
+    near = v.clone()
+    near[near < -1e30] = -2.0 ** 90 if dtype == BF16 else -6e4      # far from the end: no infinity
+    got = fa.forward_packed(q.cuda(), k.cuda(), near.cuda(), ref.offsets([nq]).cuda(), ref.offsets([nk]).cuda(), causal=causal)
+    bounds.check_prompts(got, q, k, near, [nq], [nk], causal, d ** -0.5)
+    assert bool(torch.isfinite(got).all())
+
+
+def test_decoding_with_the_lowest_values(fa):
+    lens, d = [700, 50, 3000], 128
+    kc, vc, table, rows = filled(lens, 16, 1, d, BF16, seed=8)
+    for r in rows[1]:
+        r[::9, 0, 3::7] = torch.finfo(BF16).min
+    ref.fill(vc, table, rows[1], 16)
+    q = torch.randn(3, 4, d, generator=torch.Generator().manual_seed(1)).to(BF16)
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    bounds.check_decoding(got, q, rows, lens, d ** -0.5)
+    assert bool(torch.isfinite(got).all())
