@@ -49,13 +49,13 @@ def _hipcc():
 # no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip
 HIP_FLAGS = ["-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Translation units of the library -> (flags of its own, headers).  The attention forward on [B, H, N, d] tensors has
-# no place for NaN; the serving operators have (masked places may hold them).
+# no place for NaN; the serving operators have (masked places may hold them), and are compiled with them.
 HIP_UNITS = {
     "flash_hip": (["-fno-honor-nans"], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp",
                                         "cast_f16.hpp", "host.hpp"]),
-    "flash_packed": (["-fno-honor-nans"], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp", "attn_direct.hpp",
-                                           "attn_packed.hpp", "attn_packed_mfma.hpp", "attn_packed_mfma_body.hpp",
-                                           "serving_index.hpp", "host.hpp"]),
+    "flash_packed": ([], ["attn_fwd_mfma.hpp", "attn_fwd_mfma16.hpp", "attn_fwd_mfma16_body.hpp", "attn_direct.hpp",
+                          "attn_packed.hpp", "attn_packed_mfma.hpp", "attn_packed_mfma_body.hpp",
+                          "serving_index.hpp", "host.hpp"]),
     "flash_serve": ([], ["attn_direct.hpp", "attn_paged.hpp", "attn_packed.hpp", "cache_append.hpp",
                          "serving_index.hpp", "host.hpp"]),
 }

@@ -399,6 +399,20 @@ struct QueryLimit {
 __device__ __forceinline__ int key_limit(int N, int) { return N; }
 __device__ __forceinline__ int key_limit(const QueryLimit& l, int q) { return l.first + 64 * q; }
 
+// The running maximum of scores, and whether it exceeds the (positive) threshold: one instruction for two scores.  Units
+// that honour NaNs take it of the numbers' bits as integers, which is the same maximum where a score is positive, a negative
+// number where none is, and makes a NaN exceed the threshold (the rare path sorts the rows out).  Of results of inline asm the
+// compiler does not know that they are no signalling NaNs, and a maximum of floats would quiet each by an instruction.
+#if defined(FLASH_M16_HONOR_NANS)
+__device__ __forceinline__ float score_max(float a, float b) { return __int_as_float(max(__float_as_int(a), __float_as_int(b))); }
+__device__ __forceinline__ bool score_exceeds(float a, float thr) { return __float_as_int(a) > __float_as_int(thr); }
+#define FLASH_SCORE_LESS "v_cmp_lt_i32"
+#else
+__device__ __forceinline__ float score_max(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ bool score_exceeds(float a, float thr) { return a > thr; }
+#define FLASH_SCORE_LESS "v_cmp_lt_f32"
+#endif
+
 // One pipeline step: QK(j+1) (32 MFMAs), PV(j-1) (32 MFMAs), exp(j), in-lane max(j+1).
 //   s_cur/s_nxt[kb][q]: S^T tiles of key block kb (16 keys) and query block q (16 queries)
 //   p_prev/p_cur[q]:    P^T fragments (32 keys) of query block q
@@ -482,9 +496,7 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
   // whether ANY score of the wave exceeds the deferral threshold (the rare path works out which query
   // moved).  Value v = 8q + e is register e % 4 of tile e / 4 of query block q; op 0 folds values 0..2,
   // op u values 2u+1 and 2u+2, the last op value 31.
-  auto score = [&](int v) __attribute__((always_inline)) {
-    return v < 8 * QK0 ? -INFINITY : s_nxt[(v % 8) / 4][v / 8][v % 4];
-  };
+  auto score = [&](int v) __attribute__((always_inline)) { return s_nxt[(v % 8) / 4][v / 8][v % 4]; };
   auto max_op = [&](int u) __attribute__((always_inline)) {
     if constexpr (kKnock & 32) return;
     if constexpr (MASKED) {
@@ -496,11 +508,14 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
       }
     }
     if (u == 0) {
-      mx = fmaxf(fmaxf(score(0), score(1)), score(2));
+      mx = QK0 > 0 ? -INFINITY : score_max(score_max(score(0), score(1)), score(2));
+    } else if (2 * u + 2 < 8 * QK0) {  // blocks that take no part
+    } else if (2 * u + 2 == 8 * QK0) {
+      mx = score(2 * u + 2);
     } else if (2 * u + 2 < ELEMS) {
-      mx = fmaxf(fmaxf(mx, score(2 * u + 1)), score(2 * u + 2));
+      mx = score_max(score_max(mx, score(2 * u + 1)), score(2 * u + 2));
     } else {
-      mx = fmaxf(mx, score(ELEMS - 1));
+      mx = score_max(mx, score(ELEMS - 1));
       mx_all = mx;
       asm volatile("" : "+v"(mx_all));
       return;
@@ -574,7 +589,7 @@ __device__ __forceinline__ void pipeline_step(const Hook& hook, uint32_t kb_off,
   // out: from `pending || ballot(...)` the compiler builds the same condition out of five scalar
   // instructions, and at one wave per SIMD every instruction is issue time.
   if constexpr (HAS_QK && TRACK) {
-    asm volatile("v_cmp_lt_f32 vcc, %1, %2\n\ts_or_b64 %0, vcc, %3"
+    asm volatile(FLASH_SCORE_LESS " vcc, %1, %2\n\ts_or_b64 %0, vcc, %3"
                  : "=s"(vote)
                  : "s"(sc.thr), "v"(mx_all), "s"(pending)
                  : "vcc", "scc", "memory");
@@ -634,7 +649,7 @@ __device__ __forceinline__ void step_end(f32x4 (&o)[kQ16][NB], State (&st)[kQ16]
   if constexpr (PIN) pin_tiles(s_nxt, bias);
   if (__builtin_expect(vote != 0, 0)) {
     bool any_need = false;
-    if constexpr (HAS_NEXT) any_need = __builtin_amdgcn_ballot_w64(mx_all > sc.thr) != 0;
+    if constexpr (HAS_NEXT) any_need = __builtin_amdgcn_ballot_w64(score_exceeds(mx_all, sc.thr)) != 0;
     if (pending != 0) {
       drain_o(o);
 #pragma unroll

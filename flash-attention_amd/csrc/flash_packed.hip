@@ -1,5 +1,6 @@
-// Launch of the pipelined kernel for packed prompts.  Compiled without regard to NaN like the kernels whose body it
-// shares (fmaxf of matrix results must be one instruction); what may be NaN here is looked at through its bits.
+// Launch of the pipelined kernel for packed prompts.  Unlike the other unit that compiles the kernel's body this one is compiled
+// with NaNs: masked places may hold them, and rows that meet one are computed again here, with plain arithmetic on it.
+#define FLASH_M16_HONOR_NANS 1
 #include "../../include/flash_hip.h"
 
 #include <hip/hip_runtime.h>

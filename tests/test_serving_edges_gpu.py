@@ -213,3 +213,24 @@ def test_decoding_with_the_lowest_values(fa):
     got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
     bounds.check_decoding(got, q, rows, lens, d ** -0.5)
     assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("d,dtype,causal", [(128, BF16, True), (64, F16, True), (64, F16, False)])
+@pytest.mark.parametrize("bad", [float("nan"), -float("nan"), float("inf")])
+def test_a_query_that_is_no_number_stays_by_itself(fa, d, dtype, causal, bad):
+    """Rows that share a wave with one whose scores are NaN or infinite, while their own references have to move."""
+    n = 700
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(dtype) for h in (2, 1, 1))
+    for j, gain in ((70, 0.3), (200, 1.0), (401, 2.0), (650, 3.5)):
+        k[j] = q[j, 0] * gain
+    cu = ref.offsets([n]).cuda()
+    want = fa.forward_packed(q.cuda(), k.cuda(), v.cuda(), cu, causal=causal)
+    bounds.check_prompts(want, q, k, v, [n], [n], causal, d ** -0.5, heads=[0])
+    rows = torch.tensor([3, 77, 300, 301, 540])
+    q[rows] = bad
+    got = fa.forward_packed(q.cuda(), k.cuda(), v.cuda(), cu, causal=causal)
+    others = torch.ones(n, dtype=torch.bool)
+    others[rows] = False
+    assert torch.equal(got.cpu()[others].view(torch.int16), want.cpu()[others].view(torch.int16))
+    assert bool(torch.isnan(got.cpu()[rows]).all())

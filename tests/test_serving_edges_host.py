@@ -1,6 +1,7 @@
 """CPU only: the serving operators at the ends of what they take: the columns their loads touch, scratch and grids of calls
 of unusual shape, what their outputs must not share, tensors that carry gradients."""
 import ctypes
+import importlib.util
 import os
 import subprocess
 
@@ -60,3 +61,16 @@ def test_grids_that_no_launch_takes_are_refused(fa):
         assert refused(fa, L.flash_cache_append(ctypes.byref(x), ctypes.byref(cache()), None), "tokens")
     x = Append(**{**one_row, "k": P + 8}, tokens=(1 << 29) - 33)
     assert refused(fa, L.flash_cache_append(ctypes.byref(x), ctypes.byref(cache()), None), "16-byte")
+
+
+def test_the_serving_operators_are_compiled_with_nans():
+    """Masked places may hold NaN, and rows that see one are computed with it: no unit of theirs may be compiled as if there
+    were none.  The pipelined kernel's running maximum, which would quiet every score, is one of integers there."""
+    spec = importlib.util.spec_from_file_location("fa_build", os.path.join(ROOT, "flash-attention_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    for unit in ("flash_packed", "flash_serve"):
+        for flag in build.HIP_FLAGS + build.HIP_UNITS[unit][0]:
+            assert not any(x in flag for x in ("nans", "fast", "finite", "infinities")), (unit, flag)
+    text = open(os.path.join(ROOT, "flash-attention_amd", "csrc", "flash_packed.hip")).read()
+    assert text.index("#define FLASH_M16_HONOR_NANS") < text.index("#include")
