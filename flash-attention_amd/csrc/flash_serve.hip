@@ -52,6 +52,13 @@ int check_rows(const char* what, const void* base, int64_t outer, int64_t rows, 
   return FLASH_HIP_OK;
 }
 
+// Rows that a call writes: no element of them twice.
+int check_written(const char* what, int64_t outer, int64_t rows, int64_t inner, int64_t heads, int64_t d) {
+  REFUSE_IF(flash_hip::rows_meet({rows, outer}, {heads, inner}, {1, 0}, d), "%s: rows must not overlap in memory (strides %lld, %lld)", what,
+            (long long)outer, (long long)inner);
+  return FLASH_HIP_OK;
+}
+
 #define CHECK(call)                          \
   do {                                       \
     const int rc_ = (call);                  \
@@ -117,6 +124,7 @@ int plan_decode(const flash_decode_args* a, const flash_paged_cache* c, bool mem
   CHECK(check_scale(a->softmax_scale));
   CHECK(check_rows("q", memory ? a->q : nullptr, a->q_batch_stride, c->sequences, a->q_head_stride, a->q_heads, 2, 16));
   CHECK(check_rows("out", memory ? a->o : nullptr, a->o_batch_stride, c->sequences, a->o_head_stride, a->q_heads, 2, 16));
+  CHECK(check_written("out", a->o_batch_stride, c->sequences, a->o_head_stride, a->q_heads, c->d));
   if (memory && c->sequences > 0) REFUSE_IF(!a->q || !a->o, "null tensor pointer");
   const int64_t group = a->q_heads / c->kv_heads;
   plan->tile_d = c->d <= 64 ? 64 : 128;
@@ -180,6 +188,7 @@ int plan_packed(const flash_packed_args* a, bool memory, flash_hip::packed::Para
   CHECK(check_rows("k", memory ? a->k : nullptr, a->k_token_stride, a->total_k, a->k_head_stride, a->kv_heads, 2, 16));
   CHECK(check_rows("v", memory ? a->v : nullptr, a->v_token_stride, a->total_k, a->v_head_stride, a->kv_heads, 2, 16));
   CHECK(check_rows("out", memory ? a->o : nullptr, a->o_token_stride, a->total_q, a->o_head_stride, a->q_heads, 2, 16));
+  CHECK(check_written("out", a->o_token_stride, a->total_q, a->o_head_stride, a->q_heads, a->d));
   flash_hip::packed::Params& p = *out;
   p.q = (const char*)a->q;
   p.k = (const char*)a->k;
@@ -267,6 +276,8 @@ int flash_cache_append(const flash_append_args* a, const flash_paged_cache* c, v
             "between 0 and %lld tokens (got %lld)", (1ll << 32) / ap::kThreads * ap::kMostTokens - ap::kMostTokens - 1, (long long)a->tokens);
   REFUSE_IF(!a->cu_seqlens && a->tokens != c->sequences, "without cu_seqlens one token per sequence is needed (got %lld tokens, %lld sequences)",
             (long long)a->tokens, (long long)c->sequences);
+  REFUSE_IF(flash_hip::rows_meet({c->num_pages, c->page_stride}, {c->kv_heads, c->head_stride}, {c->page_size, c->slot_stride}, c->d),
+            "cache: rows must not overlap in memory (strides %lld, %lld, %lld)", (long long)c->page_stride, (long long)c->head_stride, (long long)c->slot_stride);
   if (a->tokens == 0 || c->sequences == 0) return FLASH_HIP_OK;
   REFUSE_IF(!a->k || !a->v, "null tensor pointer");
   CHECK(check_rows("k", a->k, a->k_token_stride, a->tokens, a->k_head_stride, c->kv_heads, 2, 16));

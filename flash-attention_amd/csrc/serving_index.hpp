@@ -18,6 +18,43 @@ FLASH_INDEX int32_t within(int32_t x, int32_t low, int32_t high) { return x < lo
 // Workgroups that one dimension of a grid can have: the runtime refuses 2^32 threads and more along it
 FLASH_INDEX bool grid_fits(uint64_t workgroups, uint32_t threads) { return workgroups < (1ull << 32) / threads; }
 
+// ---- rows that are written ----------------------------------------------------------------------------------------
+// Rows of `d` elements at every sum of i * stride, 0 <= i < count, over up to three dimensions.
+struct RowDim {
+  int64_t count, stride;
+};
+// Whether two of the rows share an element: dimensions whose strides reach over all that the smaller ones span do not add
+// to that, nor do two that interleave without meeting.  (A third one that interleaves with both counts as meeting.)
+FLASH_INDEX bool rows_meet(RowDim a, RowDim b, RowDim c, int64_t d) {
+  RowDim dims[3] = {a, b, c};
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i].count < 1) return false;  // no rows
+    if (dims[i].count == 1) dims[i].stride = 0;
+    for (int j = i; j > 0 && dims[j].stride < dims[j - 1].stride; --j) {
+      const RowDim x = dims[j];
+      dims[j] = dims[j - 1];
+      dims[j - 1] = x;
+    }
+  }
+  int64_t span = d;  // of the dimensions so far
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i].count == 1) continue;
+    if (dims[i].stride < span) {
+      const int inner = i - 1;
+      if (dims[i].stride < d || inner < 0 || span != d + (dims[inner].count - 1) * dims[inner].stride) return true;
+      // two dimensions: rows i * outer + j * inner are apart if no multiple of the outer stride comes closer than d to one of
+      // the inner stride
+      const int64_t step = dims[inner].stride, most = dims[inner].count - 1;
+      for (int64_t n = 1; n < dims[i].count && n * dims[i].stride < span; ++n) {
+        const int64_t at = n * dims[i].stride, below = at / step < most ? at / step : most;
+        if (at - below * step < d || (below < most && (below + 1) * step - at < d)) return true;
+      }
+    }
+    span += (dims[i].count - 1) * dims[i].stride;
+  }
+  return false;
+}
+
 // ---- packed sequences -------------------------------------------------------------------------------------------
 struct Range {
   int32_t start, count;

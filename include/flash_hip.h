@@ -235,7 +235,7 @@ int flash_fwd_query_entry(int64_t B, int64_t H, int64_t N, int64_t d, int kernel
  *   - offsets, lengths and page tables are device memory and are read by the kernels, so that a captured graph
  *     follows them.  Whatever they hold, nothing outside the tensors is read or written: offsets are cut to the
  *     tensors, lengths to the table's reach, and a page index outside the cache means "no keys here".
- *   - the tensors of a call do not overlap.
+ *   - the tensors of a call do not overlap, nor do the rows of one that is written (-> INVALID_ARGUMENT).
  */
 
 /* Element types.  Values of e4m3: 4 exponent and 3 mantissa bits, no infinities, largest 448. */

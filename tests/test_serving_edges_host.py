@@ -9,16 +9,18 @@ import pytest
 import torch
 
 from conftest import ROOT
-from test_serving_host import P, Append, Packed, cache, refused
+from test_serving_host import P, Append, Decode, Packed, cache, caches, packed, paged, refused
 
 F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
 
 
-def test_loads_stay_inside_their_rows(tmp_path):
-    """tests/native/serving_columns_test.cpp: the columns that decoding loads of a cache row, load widths included."""
-    exe = str(tmp_path / "serving_columns_test")
-    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all",
-                           os.path.join(ROOT, "tests", "native", "serving_columns_test.cpp"), "-o", exe])
+@pytest.mark.parametrize("name", ["serving_columns_test", "serving_overlap_test"])
+def test_index_arithmetic(tmp_path, name):
+    """tests/native/serving_columns_test.cpp: the columns that decoding loads of a cache row, load widths included;
+    serving_overlap_test.cpp: rows of an output that share an element."""
+    exe = str(tmp_path / name)
+    subprocess.check_call(["g++", "-std=c++17", "-O2", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                           os.path.join(ROOT, "tests", "native", name + ".cpp"), "-o", exe])
     out = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
 
@@ -74,3 +76,47 @@ def test_the_serving_operators_are_compiled_with_nans():
             assert not any(x in flag for x in ("nans", "fast", "finite", "infinities")), (unit, flag)
     text = open(os.path.join(ROOT, "flash-attention_amd", "csrc", "flash_packed.hip")).read()
     assert text.index("#define FLASH_M16_HONOR_NANS") < text.index("#include")
+
+
+def overlapping(shape, dtype=F16):
+    """Tensors of this shape whose rows share memory."""
+    room = torch.zeros(1 << 14, dtype=dtype)
+    dense = torch.zeros(shape, dtype=dtype).stride()
+    out = [torch.zeros((1,) + shape[1:], dtype=dtype).expand(shape)]
+    for i in range(len(shape) - 1):
+        out.append(room.as_strided(shape, dense[:i] + (0,) + dense[i + 1:]))       # one place for all of a dimension
+        out.append(room.as_strided(shape, dense[:i] + (shape[-1] // 2,) + dense[i + 1:]))  # half a row further each
+    return out
+
+
+def test_outputs_whose_rows_overlap_are_refused(fa):
+    for out in overlapping((6, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            fa.forward_packed(**packed(out=out))
+    for out in overlapping((2, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            fa.decode_paged(**paged(out=out))
+    # (the same strides are no reason to refuse what is read: these calls come as far as the device)
+    for x in overlapping((5, 2, 16, 64)):
+        with pytest.raises(ValueError, match="no CPU path"):
+            fa.decode_paged(**paged(k_cache=x, v_cache=x))
+    for out in (torch.zeros(6, 8, 64, dtype=F16)[:, ::2], torch.zeros(4, 6, 64, dtype=F16).transpose(0, 1), torch.zeros(6, 4, 72, dtype=F16)[..., :64]):
+        with pytest.raises(ValueError, match="no CPU path"):
+            fa.forward_packed(**packed(out=out))
+
+
+def test_written_caches_whose_rows_overlap_are_refused(fa):
+    L = fa.lib()
+    a = Append(k=P, v=P, tokens=2, k_token_stride=128, k_head_stride=64, v_token_stride=128, v_head_stride=64, dtype=0)
+    for change in (dict(page_stride=0), dict(head_stride=0), dict(slot_stride=0), dict(slot_stride=32), dict(head_stride=960), dict(page_stride=1024)):
+        assert refused(fa, L.flash_cache_append(ctypes.byref(a), ctypes.byref(cache(**change)), None), "overlap"), change
+    d = Decode(q=P, o=P, q_heads=4, q_batch_stride=256, q_head_stride=64, o_batch_stride=256, o_head_stride=64, softmax_scale=0.125, dtype=0)
+    assert L.flash_decode_paged_workspace_bytes(ctypes.byref(d), ctypes.byref(cache(page_stride=0))) > 0      # read only
+    for change in (dict(o_batch_stride=0), dict(o_head_stride=0), dict(o_batch_stride=192), dict(o_head_stride=56)):
+        bad = Decode(**{f: getattr(d, f) for f, _ in Decode._fields_ if f not in change}, **change)
+        assert refused(fa, L.flash_decode_paged(ctypes.byref(bad), ctypes.byref(cache()), P, 1 << 40, None), "overlap"), change
+    # layouts as caches have them: heads or tokens first, K and V side by side, a layer of several
+    for change in (dict(head_stride=64, slot_stride=128), dict(head_stride=2048, slot_stride=128, page_stride=4096),
+                   dict(page_stride=1 << 30), dict(head_stride=5 * 16 * 64, page_stride=16 * 64)):
+        y = Append(k=P, v=P, tokens=0, cu_seqlens=P, dtype=0)
+        assert L.flash_cache_append(ctypes.byref(y), ctypes.byref(cache(**change)), None) == 0
