@@ -253,7 +253,7 @@ def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = T
     Scores that are seen are meant to be finite: a query that sees a key with infinite entries may get NaN.
 
     Returns a new tensor like q, or ``out`` (apart from q, k and v in memory); rows behind the last sequence are left as
-    they were.  No backward pass.  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
+    they were.  No derivative (tensors that carry gradients are refused).  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
     return _serving("forward_packed")(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, softmax_scale=softmax_scale,
                                       out=out, sync=sync)
 

@@ -3,6 +3,7 @@
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <hip/hip_runtime_api.h>
 
 #include <cmath>
@@ -52,9 +53,14 @@ void check_int32(const Tensor& t, const char* what, int64_t dims) {
   refuse_if(t.dim() != dims, what, " must have ", dims, " dimension(s), got ", t.dim());
   refuse_if(t.size(dims - 1) > 1 && t.stride(dims - 1) != 1, what, ": entries must be adjacent");
 }
+// No tensor of a call, an output among them, takes part in a derivative: neither backward nor forward.
 void check_no_grad(std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors) refuse_if(t->requires_grad(), "there is no backward pass: detach the tensors or run under no_grad");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    refuse_if(backward && t->requires_grad(), "there is no backward pass: detach the tensors or run under no_grad");
+    refuse_if(forward && t->_fw_grad(/*level=*/0).defined(), "there is no forward-mode derivative: detach the tensors");
+  }
 }
 void check_device(const Tensor& first, std::initializer_list<const Tensor*> tensors) {
   refuse_if(!first.is_cuda(), "tensors must be on a HIP device (there is no CPU path)");
@@ -175,7 +181,7 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   refuse_if(cu_q.size(0) < 1 || cu_k.size(0) != cu_q.size(0), "cu_seqlens_q and cu_seqlens_k must have one entry more than there are sequences, got ",
             cu_q.size(0), " and ", cu_k.size(0));
   refuse_if(!cu_k_given && k.size(0) != q.size(0), "without cu_seqlens_k there must be as many keys as queries, got ", k.size(0), " and ", q.size(0));
-  check_no_grad({&q, &k, &v});
+  check_no_grad({&q, &k, &v, &or_none(out_given)});
   a.sequences = cu_q.size(0) - 1;
   a.total_q = q.size(0);
   a.total_k = k.size(0);
@@ -233,7 +239,7 @@ std::tuple<Tensor, Tensor> decode_paged(const Tensor& q, const Tensor& k_cache, 
   const flash_paged_cache c = describe(k_cache, v_cache, page_table, &seq_lens, or_none(k_scale), or_none(v_scale));
   flash_decode_args a = decode_args(q, c);
   a.softmax_scale = scale_of(softmax_scale, c.d);
-  check_no_grad({&q, &k_cache, &v_cache});
+  check_no_grad({&q, &k_cache, &v_cache, &or_none(k_scale), &or_none(v_scale), &or_none(out_given), &or_none(workspace)});
   a.o_batch_stride = a.q_heads * c.d;
   a.o_head_stride = c.d;
   if (out_given) {
@@ -277,7 +283,7 @@ void cache_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const
     refuse_if(cu_seqlens->size(0) != c.sequences + 1, "cu_seqlens must have ", c.sequences + 1, " entries, got ", cu_seqlens->size(0));
     a.cu_seqlens = static_cast<const int32_t*>(cu_seqlens->const_data_ptr());
   }
-  check_no_grad({&k, &v, &k_cache, &v_cache});
+  check_no_grad({&k, &v, &k_cache, &v_cache, &or_none(k_scale), &or_none(v_scale)});
   a.k = k.const_data_ptr();
   a.v = v.const_data_ptr();
   a.k_token_stride = k.stride(0);

@@ -4,8 +4,8 @@
 //
 // Like flash::forward they check their arguments (std::invalid_argument), run on the current HIP stream of the
 // tensors' device and, with `sync`, wait for the result.  Shapes, types and strides are checked before the device, so
-// that a refusal needs no GPU.  There is no backward pass: tensors that require a gradient are refused while
-// gradients are recorded.
+// that a refusal needs no GPU.  There is no derivative: tensors that require a gradient are refused while
+// gradients are recorded, and so are tensors with a forward-mode tangent, scales and outputs among them.
 #pragma once
 #include <torch/torch.h>
 

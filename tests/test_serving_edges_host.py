@@ -120,3 +120,39 @@ def test_written_caches_whose_rows_overlap_are_refused(fa):
                    dict(page_stride=1 << 30), dict(head_stride=5 * 16 * 64, page_stride=16 * 64)):
         y = Append(k=P, v=P, tokens=0, cu_seqlens=P, dtype=0)
         assert L.flash_cache_append(ctypes.byref(y), ctypes.byref(cache(**change)), None) == 0
+
+
+E4M3_CACHES = caches(5, 2, 16, 64, dtype=E4M3)
+
+
+@pytest.mark.parametrize("how", ["backward", "forward"])
+@pytest.mark.parametrize("call,name,tensor", [
+    ("forward_packed", "q", None), ("forward_packed", "v", None), ("forward_packed", "out", torch.zeros(6, 4, 64, dtype=F16)),
+    ("decode_paged", "q", None), ("decode_paged", "v_cache", None), ("decode_paged", "out", torch.zeros(2, 4, 64, dtype=F16)),
+    ("decode_paged", "k_scale", torch.ones(2)), ("decode_paged", "v_scale", torch.ones(2)), ("decode_paged", "workspace", torch.zeros(1 << 22)),
+    ("cache_append", "k", torch.zeros(2, 2, 64, dtype=F16)), ("cache_append", "v_cache", None), ("cache_append", "k_scale", torch.ones(2)),
+])
+def test_tensors_that_carry_gradients_are_refused(fa, call, name, tensor, how):
+    """Whatever the argument: a gradient that would not be computed, or a tangent that would be lost."""
+    a = packed() if call == "forward_packed" else paged(**(E4M3_CACHES if "scale" in name else {}))
+    if call == "cache_append":
+        a.pop("q")
+        a.update(k=torch.zeros(2, 2, 64, dtype=F16), v=torch.zeros(2, 2, 64, dtype=F16))
+    x = (a[name] if tensor is None else tensor).detach().clone()
+    run = getattr(fa, call)
+    if how == "backward":
+        a[name] = x.requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            run(**a)
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
+            run(**a)
+    else:
+        with torch.autograd.forward_ad.dual_level():
+            a[name] = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(ValueError, match="forward-mode"):
+                run(**a)
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                run(**a)
+            a[name] = x
+            with pytest.raises(ValueError, match="no CPU path"):
+                run(**a)
