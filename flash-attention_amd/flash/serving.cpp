@@ -62,6 +62,12 @@ void check_no_grad(std::initializer_list<const Tensor*> tensors) {
     refuse_if(forward && t->_fw_grad(/*level=*/0).defined(), "there is no forward-mode derivative: detach the tensors");
   }
 }
+// Tensors that the call writes are modified, for whoever saved them (those of inference mode keep no count)
+void modified(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) {
+    if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+}
 void check_device(const Tensor& first, std::initializer_list<const Tensor*> tensors) {
   refuse_if(!first.is_cuda(), "tensors must be on a HIP device (there is no CPU path)");
   for (const Tensor* t : tensors) refuse_if(t->defined() && t->device() != first.device(), "tensors on different devices");
@@ -219,6 +225,7 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   Tensor scratch;
   if (need > 0) scratch = stream_workspace(q.device(), stream, need, {0, FLASH_PACKED_TICKET_BYTES});
   raise(flash_fwd_packed(&a, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
+  modified({&or_none(out_given)});
   if (sync) wait_for(stream);
   return o;
 }
@@ -263,6 +270,7 @@ std::tuple<Tensor, Tensor> decode_paged(const Tensor& q, const Tensor& k_cache, 
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
   if (need > 0) scratch = workspace ? *workspace : stream_workspace(q.device(), stream, need, {FLASH_DECODE_PARTS_BYTES, -1});
   raise(flash_decode_paged(&a, &c, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
+  modified({&or_none(out_given), &or_none(workspace)});
   if (sync) wait_for(stream);
   return {o, lse};
 }
@@ -294,6 +302,7 @@ void cache_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(k.device());
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(k.device().index());
   raise(flash_cache_append(&a, &c, stream.stream()));
+  modified({&k_cache, &v_cache});
   if (sync) wait_for(stream);
 }
 

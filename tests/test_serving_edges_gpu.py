@@ -234,3 +234,37 @@ def test_a_query_that_is_no_number_stays_by_itself(fa, d, dtype, causal, bad):
     others[rows] = False
     assert torch.equal(got.cpu()[others].view(torch.int16), want.cpu()[others].view(torch.int16))
     assert bool(torch.isnan(got.cpu()[rows]).all())
+
+
+def test_writes_are_seen_by_autograd(fa):
+    """An output, a cache or scratch that was saved for a backward pass and is then written counts as modified in place;
+    tensors of inference mode, which have no version, are taken."""
+    cu = torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+    one = torch.tensor([3], dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, 200, dtype=torch.int32, device="cuda")
+    q = torch.ones(6, 2, 64, dtype=F16, device="cuda")
+
+    def tensors():
+        return (torch.zeros(6, 2, 64, dtype=F16, device="cuda"), torch.zeros(1, 2, 64, dtype=F16, device="cuda"),
+                torch.zeros(2, 2, 16, 64, dtype=F16, device="cuda"), torch.zeros(2, 2, 16, 64, dtype=F16, device="cuda"),
+                torch.zeros(1 << 24, dtype=torch.uint8, device="cuda"))
+
+    def calls(out, step, kc, vc, scratch):
+        return ((lambda: fa.forward_packed(q, q, q, cu, out=out), [out]), (lambda: fa.cache_append(q[:1], q[:1], kc, vc, table, one), [kc, vc]),
+                (lambda: fa.decode_paged(q[:1], kc, vc, table, one, out=step, workspace=scratch), [step, scratch]))
+
+    for call, written in calls(*tensors()):
+        before = [t._version for t in written]
+        saved = written[0]
+        w = torch.ones_like(saved, requires_grad=True)
+        product = (w * saved).sum()
+        call()
+        assert all(t._version > v for t, v in zip(written, before))
+        assert [t._version for t in (q, cu, table, one)] == [0, 0, 0, 0]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    with torch.inference_mode():
+        made = tensors()
+    for call, written in calls(*made):
+        call()
+        assert bool(torch.isfinite(written[0].float()).all())
