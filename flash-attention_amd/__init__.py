@@ -225,16 +225,18 @@ def load_pyflash() -> None:
 # ---- serving: packed prompts, a paged key-value cache, one new token at a time ----------------------
 # No counterpart in the reference.  The checks and the launch are in C++ (flash/serving.cpp, reached through
 # torch.ops.pyflash.*): a decoding step is a few microseconds of GPU time, which ctypes would double.
-_serving_ops: Dict[str, Any] = {}
+_serving_ops: Dict[Tuple[str, str], Any] = {}
 
 
-def _serving(name: str):
-    op = _serving_ops.get(name)
+def _serving(name: str, out=None):
+    """The operator ``name``; with an output given, its form that returns it."""
+    form = "default" if out is None else "out"
+    op = _serving_ops.get((name, form))
     if op is None:
         import torch
 
         load_pyflash()
-        op = _serving_ops[name] = getattr(torch.ops.pyflash, name).default
+        op = _serving_ops[name, form] = getattr(getattr(torch.ops.pyflash, name), form)
     return op
 
 
@@ -254,8 +256,9 @@ def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = T
 
     Returns a new tensor like q, or ``out`` (apart from q, k and v in memory); rows behind the last sequence are left as
     they were.  No derivative (tensors that carry gradients are refused).  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
-    return _serving("forward_packed")(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, softmax_scale=softmax_scale,
-                                      out=out, sync=sync)
+    given = {} if out is None else {"out": out}
+    return _serving("forward_packed", out)(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, softmax_scale=softmax_scale,
+                                           sync=sync, **given)
 
 
 def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=None, k_scale=None, v_scale=None, out=None,
@@ -275,8 +278,9 @@ def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=Non
     callers that manage memory themselves; it serves any number of calls one after the other, calls that may overlap
     need one each.  (Without it, calls on a stream share one that is kept for the stream, and a captured graph gets its
     own.)  Lengths and pages are read on the device, so a captured graph follows them."""
-    o, lse = _serving("decode_paged")(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, k_scale=k_scale,
-                                      v_scale=v_scale, out=out, return_lse=return_lse, workspace=workspace, sync=sync)
+    given = {} if out is None else {"out": out}
+    o, lse = _serving("decode_paged", out)(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, k_scale=k_scale,
+                                           v_scale=v_scale, return_lse=return_lse, workspace=workspace, sync=sync, **given)
     return (o, lse) if return_lse else o
 
 

@@ -4,6 +4,7 @@
 //   torch.ops.load_library("build/pyflash/libpyflash.so")   (reference benchmarks/bench.py:12-14)
 #include <torch/extension.h>
 
+#include <optional>
 #include <string>
 
 #include "../flash/launch.hpp"
@@ -26,6 +27,11 @@ void bind(torch::Library& m, const char* op_name) {
   m.def(schema.c_str(), &attention_op<KT>);
 }
 
+using torch::Tensor;
+using Maybe = std::optional<Tensor>;
+// (None arrives as an undefined tensor)
+Maybe given(const Tensor& out) { return out.defined() ? Maybe(out) : std::nullopt; }
+
 }  // namespace
 
 TORCH_LIBRARY(pyflash, m) {
@@ -44,13 +50,29 @@ TORCH_LIBRARY(pyflash, m) {
   bind<KT::mma_qreg_async>(m, "mma_qreg_async");
 
   // the serving operators (flash/serving.hpp); no counterpart in the reference
+  // (an operator's result aliases the output it was given: a form of its own, so that the other one's is a new tensor)
   m.def("forward_packed(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor? cu_seqlens_k=None, *, bool causal=True, "
-        "float? softmax_scale=None, Tensor(a!)? out=None, bool sync=True) -> Tensor",
-        &flash::forward_packed);
+        "float? softmax_scale=None, bool sync=True) -> Tensor",
+        [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Maybe& cu_k, bool causal, std::optional<double> scale,
+           bool sync) { return flash::forward_packed(q, k, v, cu_q, cu_k, causal, scale, std::nullopt, sync); });
+  m.def("forward_packed.out(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor? cu_seqlens_k=None, *, bool causal=True, "
+        "float? softmax_scale=None, Tensor(a!) out, bool sync=True) -> Tensor(a!)",
+        [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Maybe& cu_k, bool causal, std::optional<double> scale,
+           const Tensor& out, bool sync) { return flash::forward_packed(q, k, v, cu_q, cu_k, causal, scale, given(out), sync); });
   m.def("decode_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor seq_lens, *, "
-        "float? softmax_scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, bool return_lse=False, "
+        "float? softmax_scale=None, Tensor? k_scale=None, Tensor? v_scale=None, bool return_lse=False, "
         "Tensor(b!)? workspace=None, bool sync=True) -> (Tensor, Tensor)",
-        &flash::decode_paged);
+        [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lens, std::optional<double> scale,
+           const Maybe& k_scale, const Maybe& v_scale, bool lse, const Maybe& workspace, bool sync) {
+          return flash::decode_paged(q, k, v, table, lens, scale, k_scale, v_scale, std::nullopt, lse, workspace, sync);
+        });
+  m.def("decode_paged.out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor seq_lens, *, "
+        "float? softmax_scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!) out, bool return_lse=False, "
+        "Tensor(b!)? workspace=None, bool sync=True) -> (Tensor(a!), Tensor)",
+        [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lens, std::optional<double> scale,
+           const Maybe& k_scale, const Maybe& v_scale, const Tensor& out, bool lse, const Maybe& workspace, bool sync) {
+          return flash::decode_paged(q, k, v, table, lens, scale, k_scale, v_scale, given(out), lse, workspace, sync);
+        });
   m.def("decode_workspace_bytes(Tensor q, Tensor k_cache, Tensor page_table) -> int", &flash::decode_workspace_bytes);
   m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor seq_lens, "
         "Tensor? cu_seqlens=None, *, Tensor? k_scale=None, Tensor? v_scale=None, bool sync=True) -> ()",

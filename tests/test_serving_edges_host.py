@@ -156,3 +156,25 @@ def test_tensors_that_carry_gradients_are_refused(fa, call, name, tensor, how):
             a[name] = x
             with pytest.raises(ValueError, match="no CPU path"):
                 run(**a)
+
+
+@pytest.mark.parametrize("name", ["forward_packed", "decode_paged"])
+def test_schemas_say_what_results_alias(fa, name):
+    """A result is a new tensor, or, in the form of its own that takes an output, that output."""
+    fa.load_pyflash()
+    op = getattr(torch.ops.pyflash, name)
+    assert not any(a.name == "out" for a in op.default._schema.arguments)
+    assert all(r.alias_info is None for r in op.default._schema.returns)
+    given = next(a for a in op.out._schema.arguments if a.name == "out")
+    result = op.out._schema.returns[0]
+    assert given.alias_info.is_write and result.alias_info.is_write
+    assert given.alias_info.before_set == result.alias_info.before_set
+    assert all(r.alias_info is None for r in op.out._schema.returns[1:])
+    # every way of calling it comes as far as the device
+    a = packed() if name == "forward_packed" else paged()
+    for more in ({}, {"out": None}, {"out": torch.zeros_like(a["q"])}):
+        for call in (op, getattr(fa, name)):
+            with pytest.raises(ValueError, match="no CPU path"):
+                call(*a.values(), **more)
+    with pytest.raises(ValueError, match="out must have"):
+        op(*a.values(), out=torch.zeros(1, 4, 64, dtype=F16))
