@@ -87,7 +87,15 @@ void wait_for(const c10::hip::HIPStreamMasqueradingAsCUDA& stream) {
 // kind of scratch has one value of zeros.first.  Work on one stream runs in order, so its calls share a buffer that is filled
 // once, on their first call (and again when a larger one is needed).  A graph under capture gets one of its own, filled by a
 // node of the graph: it may be replayed on any stream, beside any other.  So does a call on a stream that torch did not
-// make, whose handle may come to stand for another stream.
+// make, whose handle may come to stand for another stream.  Buffers are kept until release_workspaces().
+struct Kept {
+  std::mutex mutex;
+  std::map<std::tuple<int, c10::StreamId, int64_t>, Tensor> buffers;
+};
+Kept& kept() {
+  static auto& all = *new Kept;  // (never destroyed: the allocator may be gone by then)
+  return all;
+}
 Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradingAsCUDA& stream, int64_t need, std::pair<int64_t, int64_t> zeros) {
   const auto options = at::TensorOptions().dtype(at::kByte).device(device);
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -100,11 +108,8 @@ Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradin
     return t;
   };
   if (capture != hipStreamCaptureStatusNone || !own_stream) return fresh(need);
-  static std::mutex mutex;
-  // (never destroyed: the allocator may be gone by then)
-  static auto& buffers = *new std::map<std::tuple<int, c10::StreamId, int64_t>, Tensor>;
-  const std::lock_guard<std::mutex> lock(mutex);
-  Tensor& t = buffers[{device.index(), id, zeros.first}];
+  const std::lock_guard<std::mutex> lock(kept().mutex);
+  Tensor& t = kept().buffers[{device.index(), id, zeros.first}];
   if (!t.defined() || t.numel() < need) t = fresh(need + (1 << 16));
   return t;
 }
@@ -228,6 +233,12 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   modified({&or_none(out_given)});
   if (sync) wait_for(stream);
   return o;
+}
+
+void release_workspaces() {
+  decltype(Kept::buffers) all;  // (freed when the lock is given back)
+  const std::lock_guard<std::mutex> lock(kept().mutex);
+  all.swap(kept().buffers);
 }
 
 int64_t decode_workspace_bytes(const Tensor& q, const Tensor& k_cache, const Tensor& page_table) {

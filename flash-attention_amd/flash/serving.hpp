@@ -34,6 +34,10 @@ std::tuple<torch::Tensor, torch::Tensor> decode_paged(
     const std::optional<torch::Tensor>& workspace, bool sync);
 int64_t decode_workspace_bytes(const torch::Tensor& q, const torch::Tensor& k_cache, const torch::Tensor& page_table);
 
+// Gives the scratch that is kept for streams back to torch's allocator, which hands it out again in the order of each
+// stream: calls that are still running keep what they use.  Later calls allocate anew; captured graphs have their own.
+void release_workspaces();
+
 // k and v [tokens, Hkv, d] into the caches, in place.
 void cache_append(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_cache,
                   const torch::Tensor& v_cache, const torch::Tensor& page_table, const torch::Tensor& seq_lens,

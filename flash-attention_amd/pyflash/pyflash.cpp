@@ -73,6 +73,7 @@ TORCH_LIBRARY(pyflash, m) {
            const Maybe& k_scale, const Maybe& v_scale, const Tensor& out, bool lse, const Maybe& workspace, bool sync) {
           return flash::decode_paged(q, k, v, table, lens, scale, k_scale, v_scale, given(out), lse, workspace, sync);
         });
+  m.def("release_workspaces() -> ()", &flash::release_workspaces);
   m.def("decode_workspace_bytes(Tensor q, Tensor k_cache, Tensor page_table) -> int", &flash::decode_workspace_bytes);
   m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor seq_lens, "
         "Tensor? cu_seqlens=None, *, Tensor? k_scale=None, Tensor? v_scale=None, bool sync=True) -> ()",

@@ -268,3 +268,41 @@ def test_writes_are_seen_by_autograd(fa):
     for call, written in calls(*made):
         call()
         assert bool(torch.isfinite(written[0].float()).all())
+
+
+def test_scratch_of_streams_is_given_back(fa):
+    """What calls keep for their streams returns to the allocator; calls that run meanwhile and a captured one are not disturbed."""
+    fa.release_workspaces()
+    lens = [3000, 1200]
+    kc, vc, table, _ = filled(lens, 16, 2, 128, F16, seed=33)
+    gen = torch.Generator().manual_seed(1)
+    args = (torch.randn(2, 4, 128, generator=gen).half().cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    q, k, v = (torch.randn(n, h, 128, generator=gen).half().cuda() for n, h in ((130, 2), (4200, 1), (4200, 1)))
+    cus = ref.offsets([130]).cuda(), ref.offsets([4200]).cuda()
+    streams = [torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+    want = fa.decode_paged(*args), fa.forward_packed(q, k, v, *cus)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        captured = fa.decode_paged(*args, sync=False), fa.forward_packed(q, k, v, *cus, sync=False)
+    fa.release_workspaces()
+    before = torch.cuda.memory_allocated()
+    got = []
+    for turn in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((fa.decode_paged(*args, sync=False), fa.forward_packed(q, k, v, *cus, sync=False)))
+        graph.replay()
+        if turn % 2 == 1:
+            fa.release_workspaces()
+            other = [torch.full((1 << 24,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]     # takes freed memory
+            del other
+    torch.cuda.synchronize()
+    for x in got + [captured]:
+        assert all(torch.equal(a, b) for a, b in zip(x, want))
+    outputs = sum(t.untyped_storage().nbytes() for x in got for t in x)
+    assert torch.cuda.memory_allocated() - before < outputs + (1 << 20)
+    fa.decode_paged(*args)
+    assert torch.cuda.memory_allocated() - before > 10 << 20
+    fa.release_workspaces()
+    assert torch.cuda.memory_allocated() - before < outputs + (1 << 20)

@@ -178,3 +178,8 @@ def test_schemas_say_what_results_alias(fa, name):
                 call(*a.values(), **more)
     with pytest.raises(ValueError, match="out must have"):
         op(*a.values(), out=torch.zeros(1, 4, 64, dtype=F16))
+
+
+def test_releasing_scratch_needs_no_device(fa):
+    fa.release_workspaces()
+    fa.release_workspaces()
