@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     const char* src = p.q + (int64_t)b * p.q_batch + (int64_t)(kvh * p.group + row0 + (n < rows ? n : 0)) * p.q_head;
 #pragma unroll
     for (int ks = 0; ks < S::kKS; ++ks) {
-      const int col = S::column(ks, g);
-      const bool there = n < rows && (FULL || col < p.d);
+      const int col = FULL ? S::column(ks, g) : q_column(CACHE8, ks, g, p.d);
+      const bool there = n < rows && (FULL || col >= 0);
       const u32x4 x = *(const u32x4*)(src + (there ? col * 2 : 0));
       qf[ks] = there ? x : u32x4{0u, 0u, 0u, 0u};
     }
@@ -174,8 +174,22 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     uint32_t k_row = (uint32_t)n * slot_stride, v_row[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v_row[j] = (uint32_t)(4 * g + j) * slot_stride + (FULL || n * S::kE < p.d ? (uint32_t)(n * S::kE * S::kElem) : 0u);
+    // A load never leaves its row: 16 bytes of 8-bit values may be 8 columns more than the row has from there on.  Such a load
+    // begins earlier, and the query's elements stand beside the columns that it holds (q_column).
     auto load_k = [&](typename S::KBlock& k, int64_t at) __attribute__((always_inline)) {
       if constexpr (PAGE16) asm volatile("" : "+v"(k_row));
+      if constexpr (!FULL && CACHE8) {
+        if (p.d == 8) {  // rows shorter than a load
+#pragma unroll
+          for (int t = 0; t < 2 * NS; ++t) {
+            const char* src = PAGE16 ? kh + tile_start(at, t) + k_row : kh + __shfl(at, 16 * t + n);
+            const u32x2 x = stream((const u32x2*)src);
+#pragma unroll
+            for (int i = 0; i < S::kKLoads; ++i) k[t][i] = u32x4{x[0], x[1], 0u, 0u};
+          }
+          return;
+        }
+      }
 #pragma unroll
       for (int t = 0; t < 2 * NS; ++t) {
         const char* src = PAGE16 ? kh + tile_start(at, t) : kh + __shfl(at, 16 * t + n);
@@ -183,19 +197,12 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
         for (int i = 0; i < S::kKLoads; ++i) {
           if constexpr (PAGE16 && FULL) {
             k[t][i] = stream((const u32x4*)(src + (k_row + (uint32_t)(S::load_column(0, g) * S::kElem)) + S::load_column(i, 0) * S::kElem));
-          } else if constexpr (FULL) {
-            k[t][i] = stream((const u32x4*)(src + (uint32_t)(S::load_column(i, g) * S::kElem)));
           } else {
-            // (a load never leaves its row: 16 bytes of 8-bit values may be 8 columns more than the row has from there on)
-            constexpr int kWide = 16 / S::kElem;
-            const uint32_t row = PAGE16 ? k_row : 0u;
-            if (kWide > 8 && p.d == 8) {
-              const u32x2 x = stream((const u32x2*)(src + row));
-              k[t][i] = S::load_column(i, g) == 0 ? u32x4{x[0], x[1], 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
-            } else {
-              const RowLoad at_row = row_load(S::load_column(i, g), kWide, p.d);
-              const u32x4 x = stream((const u32x4*)(src + (row + (uint32_t)(at_row.from * S::kElem))));
-              k[t][i] = at_row.skip == 0 ? x : at_row.skip == kWide ? u32x4{0u, 0u, 0u, 0u} : u32x4{x[2], x[3], 0u, 0u};
+            const int col = S::load_column(i, g), from = FULL ? col : row_load(col, 16 / S::kElem, p.d);
+            k[t][i] = stream((const u32x4*)(src + ((PAGE16 ? k_row : 0u) + (uint32_t)(from * S::kElem))));
+            // (infinite elements of a 16-bit row times a query's zero would be NaN; e4m3 has none)
+            if constexpr (!FULL && !CACHE8) {
+              if (col >= p.d) k[t][i] = u32x4{0u, 0u, 0u, 0u};
             }
           }
         }

@@ -144,15 +144,15 @@ FLASH_INDEX int32_t cache_length(const Pages& c, int32_t len) { return within(le
 // first of the 8 head-dim elements that lane group g multiplies in k-step ks; a 16-byte load of an 8-bit row holds
 // those of two k-steps
 FLASH_INDEX int32_t k_column(bool cache8, int32_t ks, int32_t g) { return cache8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
-// A load of `width` elements (at most d) where the lane wants those from `column` on: where it begins, inside the row at
-// both ends, and how many elements it skips (`width`: the row has none of them; they count as zeros).
-struct RowLoad {
-  int32_t from, skip;
-};
-FLASH_INDEX RowLoad row_load(int32_t column, int32_t width, int32_t d) {
-  if (column >= d) return RowLoad{0, width};
-  const int32_t from = column + width <= d ? column : d - width;
-  return RowLoad{from, column - from};
+// Where a load of `width` elements (at most d) begins for a lane that wants those from `column` on: inside the row at both
+// ends.  What it holds in front of `column` others multiply already, or, where column >= d, all of it: no query element
+// goes with that.
+FLASH_INDEX int32_t row_load(int32_t column, int32_t width, int32_t d) { return column + width <= d ? column : d - width; }
+// The query elements that lane group g multiplies the 8 elements of k-step ks with: those from here on, -1: zeros.
+FLASH_INDEX int32_t q_column(bool cache8, int32_t ks, int32_t g, int32_t d) {
+  const int32_t wide = cache8 && d >= 16 ? 16 : 8, first = k_column(cache8, wide == 16 ? ks & ~1 : ks, g);
+  const int32_t mine = row_load(first, wide, d) + (wide == 16 ? 8 * (ks & 1) : 0);
+  return mine >= first ? mine : -1;
 }
 
 // ---- the line of units that decoding workgroups divide among themselves --------------------------------------

@@ -21,21 +21,20 @@ int main() {
   for (int d = 8; d <= 128; d += 8) {
     for (int cache8 = 0; cache8 < 2; ++cache8) {
       const int tile = d <= 64 ? 64 : 128, steps = tile / 32, wide = cache8 ? 16 : 8;
-      // K: one 16-byte load for `wide` columns (8-byte ones where a row is shorter than that)
+      // K: one 16-byte load for `wide` columns (8-byte ones where a row is shorter than that), each column of which goes
+      // with a query element at most; over all lanes and steps every one does, once
       std::vector<int> used(d, 0);
       for (int g = 0; g < 4; ++g) {
-        for (int ks = 0; ks < steps; ks += wide / 8) {
-          const int column = k_column(cache8, ks, g), width = wide <= d ? wide : 8;
-          EXPECT(!cache8 || k_column(true, ks + 1, g) == column + 8);
-          for (int c = column; c < column + wide; c += width) {   // (once, but for rows of 8 elements)
-            const RowLoad x = row_load(c, width, d);
-            EXPECT(x.from >= 0 && x.from + width <= d);
-            EXPECT(x.skip == 0 || x.skip == width || (wide == 16 && x.skip == 8));
-            for (int e = x.skip; e < width; ++e) {
-              EXPECT(x.from + e == c + e - x.skip);
-              used[x.from + e] += 1;
-            }
-          }
+        for (int ks = 0; ks < steps; ++ks) {
+          const int width = wide <= d ? wide : 8, first = k_column(cache8, wide == 16 ? ks & ~1 : ks, g);
+          EXPECT(wide == 8 || k_column(true, ks & ~1, g) + 8 * (ks & 1) == k_column(true, ks, g));
+          const int from = width == wide ? row_load(first, width, d) : 0;  // (a short row is loaded whole)
+          EXPECT(from >= 0 && from + width <= d);
+          const int held = from + (width == 16 ? 8 * (ks & 1) : 0);         // first of the 8 elements that the step multiplies
+          const int q = q_column(cache8, ks, g, d);
+          EXPECT(q == -1 || (q == held && q + 8 <= d && q % 8 == 0));
+          if (q < 0) continue;
+          for (int e = 0; e < 8; ++e) used[q + e] += 1;
         }
       }
       for (int n : used) EXPECT(n == 1);

@@ -306,3 +306,18 @@ def test_scratch_of_streams_is_given_back(fa):
     assert torch.cuda.memory_allocated() - before > 10 << 20
     fa.release_workspaces()
     assert torch.cuda.memory_allocated() - before < outputs + (1 << 20)
+
+
+@pytest.mark.parametrize("page", [16, 2])
+@pytest.mark.parametrize("d,dtype", [(40, BF16), (72, F16), (120, BF16), (128, F16), (64, BF16), (8, F16)])
+@pytest.mark.parametrize("column", [0, -1, -8])
+def test_an_infinite_element_of_a_key(fa, page, d, dtype, column):
+    """A score of minus infinity is a weight of nothing, at head dims that leave lanes without columns too."""
+    n = 77
+    kc, vc, table, rows = filled([n], page, 1, d, dtype, seed=d)
+    q = torch.randn(1, 2, d, generator=torch.Generator().manual_seed(1)).abs().to(dtype)
+    rows[0][0][[5, 40, 76], 0, column] = -float("inf")
+    ref.fill(kc, table, rows[0], page)
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
+    keep = [j for j in range(n) if j not in (5, 40, 76)]
+    bounds.check_decoding(got, q, [[r[0][keep]] for r in rows], [len(keep)], d ** -0.5)
