@@ -108,7 +108,7 @@ int launch(packed::Params p, void* workspace, hipStream_t stream) {
 static_assert(m16::kThreads == m16h::kThreads, "one limit of the grid");
 bool packed_mfma_takes(const packed::Params& p) {
   const int64_t most = (int64_t)kOob / m16::kPackedRows;  // a row's bytes: 256 of them stay below kOob
-  const int64_t tiles = (int64_t)p.total_q / m16h::kPackedRows + 2 * (int64_t)p.sequences;
+  const int64_t tiles = (int64_t)p.total_q / (take_half(p) ? m16h::kPackedRows : m16::kPackedRows) + (int64_t)extra_tiles(p) * p.sequences;
   return p.q_token <= most && p.o_token <= most && p.k_token <= most && p.v_token <= most && tiles < ((int64_t)1 << 31) &&
          grid_fits(packed_grid((uint64_t)tiles, (uint32_t)p.heads, (uint32_t)p.kv_heads), m16::kThreads);
 }

@@ -57,9 +57,11 @@ def test_as_many_keys_as_queries_with_offsets_of_their_own(fa, heads, lens):
     ref.check_packed(got, q, k, v, lens, k_lens, True, d ** -0.5, heads=[0, heads - 1])
 
 
-def test_more_short_prompts_than_one_dimension_of_a_grid_holds(fa):
-    """2^19 prompts of a row or two, 32 heads: over 2^24 (prompt, head) pairs."""
-    heads, d, sequences = 32, 8, 1 << 19
+@pytest.mark.parametrize("sequences,own_offsets", [(1 << 19, False), (400000, False), (400000, True)])
+def test_more_short_prompts_than_one_dimension_of_a_grid_holds(fa, sequences, own_offsets):
+    """Prompts of a row or two, 32 heads: over 2^24 (prompt, head) pairs, or, with two places for each prompt, twice as many
+    as are there, on either side of that."""
+    heads, d = 32, 8
     lens = torch.ones(sequences, dtype=torch.int64)
     lens[5::1000] = 0
     lens[7::997] = 2
@@ -69,7 +71,8 @@ def test_more_short_prompts_than_one_dimension_of_a_grid_holds(fa):
     q = torch.randn(total, heads, d, generator=gen, device="cuda").to(BF16)
     k, v = (torch.randn(total, 1, d, generator=gen, device="cuda").to(BF16) for _ in range(2))
     cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
-    got = fa.forward_packed(q, k, v, cu.to(torch.int32).cuda())
+    cu_q = cu.to(torch.int32).cuda()
+    got = fa.forward_packed(q, k, v, cu_q, cu_q.clone() if own_offsets else None)
     ref.check_packed(got[:203], q[:203], k[:203], v[:203], [70, 3, 0, 130], [70, 3, 0, 130], True, d ** -0.5, heads=[0, 31])
     first = cu[:-1][lens > 0].cuda()            # a prompt's first row sees itself alone
     assert torch.equal(got[first], v[first].expand(-1, heads, -1))
