@@ -252,7 +252,8 @@ def forward_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal: bool = T
     the keys j <= i + nk - nq: the last query sees the last key, which is what a later piece of a prompt needs.  A
     query that sees no key gets zeros.  Masked keys and values may hold anything, NaN and infinities included; values
     that are seen are summed in fp32 before they are divided by the weights' sum (bf16 values beyond 1e30 may overflow).
-    Scores that are seen are meant to be finite: a query that sees a key with infinite entries may get NaN.
+    Scores that are seen are meant to be finite: a query that sees a key with infinite entries may get NaN, and so may
+    one that sees an infinite value with a weight below 2^-32 of its largest.
 
     Returns a new tensor like q, or ``out`` (apart from q, k and v in memory); rows behind the last sequence are left as
     they were.  No derivative (tensors that carry gradients are refused).  Blocks until done unless ``sync=False`` (which a graph capture needs)."""
@@ -276,8 +277,8 @@ def decode_paged(q, k_cache, v_cache, page_table, seq_lens, *, softmax_scale=Non
     ``(out, lse)``, lse float32 ``[sequences, Hq]`` the logarithm of the weights' sum (-inf for length 0), with which
     results over several parts of a context can be joined.  ``workspace``: scratch from :func:`decode_workspace`, for
     callers that manage memory themselves; it serves any number of calls one after the other, calls that may overlap
-    need one each.  (Without it, calls on a stream share one that is kept for the stream, and a captured graph gets its
-    own.)  Lengths and pages are read on the device, so a captured graph follows them."""
+    need one each.  (Without it, calls on a stream share one that is kept for the stream until
+    :func:`release_workspaces`, and a captured graph gets its own.)  ``out`` lies apart from the other tensors in memory.  Lengths and pages are read on the device, so a captured graph follows them."""
     given = {} if out is None else {"out": out}
     o, lse = _serving("decode_paged", out)(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, k_scale=k_scale,
                                            v_scale=v_scale, return_lse=return_lse, workspace=workspace, sync=sync, **given)
@@ -310,7 +311,7 @@ def cache_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, 
     k and v ``[tokens, Hkv, d]``, fp16 or bf16; rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32, on the
     device; default: one row for each sequence) are the last tokens of sequence b, whose length ``seq_lens[b]`` counts
     them already.  A 16-bit cache gets the values as they are, a float8_e4m3fn cache the nearest value to
-    ``x / scale`` (ties to even, at most 448).  Rows of no sequence, positions outside the table and pages outside
+    ``x / scale`` (ties to even, at most 448).  The two caches lie apart in memory, and so do their rows.  Rows of no sequence, positions outside the table and pages outside
     the cache are not written."""
     _serving("cache_append")(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens, k_scale=k_scale, v_scale=v_scale, sync=sync)
 

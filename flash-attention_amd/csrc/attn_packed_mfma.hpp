@@ -3,7 +3,7 @@
 //
 // What bounds it: 4 d operations for each visible (query, key) pair, on the matrix cores; K and V are read from the L2s by
 // every item.  One prompt of 16384 rows, 32 heads of 128 over 8, bf16: 1.71 ms, 1290 TFLOP/s (8192^3 library product on the
-// same chip: 1261); 13 ragged ones of 0 to 2048 rows 123 us (floor 80: the diagonal's masked tiles, starts and ends).
+// same chip: 1261); 13 ragged ones of 0 to 2048 rows 122 us (floor 80; the matrix cores are busy 43 % of the time: starts and ends of items).
 //
 // The causal square is cut where the matrix tiles are: an item's first row is placed so that its last visible key ends
 // a 64-key tile (the first item of a sequence may be shorter).  Wave w holds, as query block q, the rows
@@ -11,6 +11,10 @@
 // every wave, whole by the blocks behind it and not at all by those before it: the steps of tile T leave the first T
 // blocks out and mask one, with the same work for every wave.  The diagonal then costs 2.5 tiles of matrix time
 // instead of 4 (rows in consecutive blocks per wave would make the last wave do all four).
+//
+// P enters the second product rounded to the tensors' 16-bit type (half a step of each weight), as in the operators for equal
+// lengths: a second product for what the rounding leaves would cost a third of the rate.  Its sum l is taken of the rounded
+// weights.
 //
 // Values of keys that some rows of a tile do not see are multiplied by 0 there; where they are infinite or NaN that is
 // wrong, and such rows come out as NaN.  A wave whose output holds one looks at the values of its diagonal tiles and, if

@@ -5,8 +5,8 @@
 // 2 * d * kv_heads * (2 + bytes of a cache element) bytes a token.  A workgroup takes `tokens` consecutive ones:
 // their targets are looked up once (the sequence by bisection of cu, in LDS where it fits) and every lane then moves
 // chunks of 8 elements, 16-byte loads, with consecutive lanes on consecutive chunks of a token's row.
-// Measured: 8509 tokens of 13 prompts, 8 heads of 128, 16-bit: 13-14 us, 4.9-5.3 TB/s read and written (a large copy: 4.6); 16
-// single tokens into an e4m3 cache: 3.3 us, a launch and a chain of three loads.
+// Measured: 8509 tokens of 13 prompts, 8 heads of 128, 16-bit: 13-14 us, 4.9-5.3 TB/s read and written (a large copy: 4.6),
+// into e4m3 19 us; 16 single tokens into an e4m3 cache: 3.3 us, a launch and a chain of three loads.
 // Tokens outside every sequence, positions beyond the table and pages outside the cache are not written.
 #pragma once
 

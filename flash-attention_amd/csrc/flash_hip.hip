@@ -772,7 +772,7 @@ const char* flash_kernel_type_name(int kernel_type) {
 
 const char* flash_hip_last_error(void) { return g_err; }
 
-int flash_hip_version(void) { return 400; }
+int flash_hip_version(void) { return 401; }
 
 int flash_hip_reload_switches(void) {
   publish_switches();

@@ -343,8 +343,8 @@ const char* flash_kernel_type_name(int kernel_type);
  * failing call on the same thread. */
 const char* flash_hip_last_error(void);
 
-/* Library version, major*10000 + minor*100 + patch.  400 (packed prompts, decoding over a paged cache; nothing
- * that was there changed); flash_launch_info unchanged since 200 (which
+/* Library version, major*10000 + minor*100 + patch.  401 (400: packed prompts, decoding over a paged cache; nothing
+ * that was there changed.  401: written tensors whose rows overlap and calls that no grid holds are refused); flash_launch_info unchanged since 200 (which
  * appended `persistent`: callers built against 100 must be recompiled, the query functions write the
  * whole structure). */
 int flash_hip_version(void);
