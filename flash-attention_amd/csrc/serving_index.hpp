@@ -23,6 +23,11 @@ FLASH_INDEX bool grid_fits(uint64_t workgroups, uint32_t threads) { return workg
 struct RowDim {
   int64_t count, stride;
 };
+// elements from the first row of a dimension to its last one, up to 2^61
+FLASH_INDEX int64_t row_reach(RowDim x) {
+  constexpr int64_t kMost = (int64_t)1 << 61;
+  return x.stride > 0 && x.count - 1 > kMost / x.stride ? kMost : (x.count - 1) * x.stride;
+}
 // Whether two of the rows share an element: dimensions whose strides reach over all that the smaller ones span do not add
 // to that, nor do two that interleave without meeting.  (A third one that interleaves with both counts as meeting.)
 FLASH_INDEX bool rows_meet(RowDim a, RowDim b, RowDim c, int64_t d) {
@@ -41,7 +46,7 @@ FLASH_INDEX bool rows_meet(RowDim a, RowDim b, RowDim c, int64_t d) {
     if (dims[i].count == 1) continue;
     if (dims[i].stride < span) {
       const int inner = i - 1;
-      if (dims[i].stride < d || inner < 0 || span != d + (dims[inner].count - 1) * dims[inner].stride) return true;
+      if (dims[i].stride < d || inner < 0 || span != d + row_reach(dims[inner])) return true;
       // two dimensions: rows i * outer + j * inner are apart if no multiple of the outer stride comes closer than d to one of
       // the inner stride
       const int64_t step = dims[inner].stride, most = dims[inner].count - 1;
@@ -50,7 +55,7 @@ FLASH_INDEX bool rows_meet(RowDim a, RowDim b, RowDim c, int64_t d) {
         if (at - below * step < d || (below < most && (below + 1) * step - at < d)) return true;
       }
     }
-    span += (dims[i].count - 1) * dims[i].stride;
+    span += row_reach(dims[i]);
   }
   return false;
 }

@@ -49,6 +49,12 @@ int main() {
   }
   if (meet < 1000 || apart < 1000 || extra > meet / 5) return printf("%ld %ld %ld\n", meet, apart, extra), 1;
   if (!rows_meet({1 << 30, 0}, {1, 0}, {1, 0}, 8) || rows_meet({1 << 30, (int64_t)1 << 20}, {65535, 16}, {1, 0}, 16)) return 1;
+  // sizes that no memory holds
+  for (int64_t big : {(int64_t)1 << 40, ((int64_t)1 << 40) - 8}) {
+    if (rows_meet({1 << 30, big}, {1 << 30, 64}, {1, 0}, 64) != (((int64_t)1 << 36) > big)) return printf("large strides\n"), 1;
+    if (!rows_meet({1 << 30, big}, {1 << 30, big}, {1 << 30, big}, 8)) return printf("large strides\n"), 1;
+    if (!rows_meet({1 << 30, big}, {1 << 30, big + 8}, {1, 0}, 16)) return printf("large strides\n"), 1;
+  }
   printf("rows that meet are found\n");
   return 0;
 }
