@@ -251,7 +251,8 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
     // ---- the four waves' parts --------------------------------------------------------------------------
     const bool complete = u0 == 0 && u1 == units;
     const uint32_t slot = part_slot(blockIdx.x, c, r - u0);
-    const float vs = (CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f) * (1.f / kRaise<EK>);  // and what the weights are raised by
+    const float vs = CACHE8 && p.v_scale ? p.v_scale[kvh] : 1.f;
+    constexpr float kLower = 1.f / kRaise<EK>;  // (into the sum's inverse, apart from vs: their product may pass fp32's range)
     const float l = quad_sum(st.l);
     if (g == 0) {
       sh_ml[wave][n][0] = st.m;
@@ -284,9 +285,9 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
         }
         if (complete) {
           const int32_t head = kvh * p.group + row0 + row;
-          const float inv = l == 0.f ? 0.f : vs / l;
+          const float inv = l == 0.f ? 0.f : kLower / l, unit = l == 0.f ? 0.f : vs;
           *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)head * p.o_head + col * 2) =
-              u32x2{pack2<EK>(sum[0] * inv, sum[1] * inv), pack2<EK>(sum[2] * inv, sum[3] * inv)};
+              u32x2{pack2<EK>(sum[0] * inv * unit, sum[1] * inv * unit), pack2<EK>(sum[2] * inv * unit, sum[3] * inv * unit)};
           if (p.lse && col == 0) {
             p.lse[(int64_t)b * p.kv_heads * p.group + head] = l == 0.f ? kMinusInf : (m + log2f(l)) * 0.693147180559945309f;
           }
@@ -380,9 +381,9 @@ __global__ __launch_bounds__(kThreads, 3) void decode_kernel(const Params p) {
           __syncthreads();
           if (side == 0 && col < p.d) {
             for (int s = 1; s < sides; ++s) acc += sh_sum[s * items + x];
-            const float inv = sh_l[r8] == 0.f ? 0.f : vs / sh_l[r8];
+            const float inv = sh_l[r8] == 0.f ? 0.f : kLower / sh_l[r8], unit = sh_l[r8] == 0.f ? 0.f : vs;
             *(u32x2*)(p.o + (int64_t)b * p.o_batch + (int64_t)(kvh * p.group + row0 + 8 * q + r8) * p.o_head + col * 2) =
-                u32x2{pack2<EK>(acc[0] * inv, acc[1] * inv), pack2<EK>(acc[2] * inv, acc[3] * inv)};
+                u32x2{pack2<EK>(acc[0] * inv * unit, acc[1] * inv * unit), pack2<EK>(acc[2] * inv * unit, acc[3] * inv * unit)};
           }
           __syncthreads();
         };

@@ -324,3 +324,14 @@ def test_an_infinite_element_of_a_key(fa, page, d, dtype, column):
     got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
     keep = [j for j in range(n) if j not in (5, 40, 76)]
     bounds.check_decoding(got, q, [[r[0][keep]] for r in rows], [len(keep)], d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,scale", [(BF16, 1e33), (BF16, 3e-38), (F16, 100.0), (F16, 1e-7)])
+@pytest.mark.parametrize("lens", [[40, 0], [5000, 1]])
+def test_scales_of_values_of_any_size(fa, dtype, scale, lens):
+    """What a stored 1 stands for enters the result as it is, whatever the weights are held as."""
+    kc, vc, table, rows = filled(lens, 16, 1, 64, E4M3, seed=4)
+    q = torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    vs = torch.tensor([scale])
+    got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softmax_scale=0.005, v_scale=vs.cuda())
+    bounds.check_decoding(got, q, rows, lens, 0.005, None, vs)
