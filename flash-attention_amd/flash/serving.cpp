@@ -78,6 +78,17 @@ float scale_of(std::optional<double> given, int64_t d) {
 const Tensor kNone;
 const Tensor& or_none(const Maybe& t) { return t ? *t : kNone; }
 
+bool capturing(const c10::hip::HIPStreamMasqueradingAsCUDA& stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) throw std::runtime_error("hipStreamIsCapturing failed");
+  return status != hipStreamCaptureStatusNone;
+}
+// The stream of a call.  Waiting for it would end a capture.
+c10::hip::HIPStreamMasqueradingAsCUDA stream_of(c10::Device device, bool sync) {
+  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index());
+  refuse_if(sync && capturing(stream), "the call is captured into a graph, which cannot wait for its result: pass sync=False");
+  return stream;
+}
 void wait_for(const c10::hip::HIPStreamMasqueradingAsCUDA& stream) {
   const hipError_t e = hipStreamSynchronize(stream.stream());
   if (e != hipSuccess) throw std::runtime_error(hipGetErrorString(e));
@@ -98,8 +109,6 @@ Kept& kept() {
 }
 Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradingAsCUDA& stream, int64_t need, std::pair<int64_t, int64_t> zeros) {
   const auto options = at::TensorOptions().dtype(at::kByte).device(device);
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess) throw std::runtime_error("hipStreamIsCapturing failed");
   const c10::StreamId id = stream.unwrap().id();
   const bool own_stream = id == 0 || (id & 1) != 0;  // torch's numbering: the default stream, and the streams of its pools
   auto fresh = [&](int64_t bytes) {
@@ -107,7 +116,7 @@ Tensor stream_workspace(c10::Device device, const c10::hip::HIPStreamMasqueradin
     t.slice(0, zeros.first, zeros.second < 0 ? bytes : zeros.second).zero_();
     return t;
   };
-  if (capture != hipStreamCaptureStatusNone || !own_stream) return fresh(need);
+  if (!own_stream || capturing(stream)) return fresh(need);
   const std::lock_guard<std::mutex> lock(kept().mutex);
   Tensor& t = kept().buffers[{device.index(), id, zeros.first}];
   if (!t.defined() || t.numel() < need) t = fresh(need + (1 << 16));
@@ -219,6 +228,7 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   if (need < 0) throw std::invalid_argument(flash_hip_last_error());
   check_device(q, {&k, &v, &cu_q, &cu_k, &or_none(out_given)});
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const auto stream = stream_of(q.device(), sync);
   Tensor o = output_for(q, out_given);
   a.q = q.const_data_ptr();
   a.k = k.const_data_ptr();
@@ -226,7 +236,6 @@ Tensor forward_packed(const Tensor& q, const Tensor& k, const Tensor& v, const T
   a.o = o.data_ptr();
   a.cu_seqlens_q = static_cast<const int32_t*>(cu_q.const_data_ptr());
   a.cu_seqlens_k = static_cast<const int32_t*>(cu_k.const_data_ptr());
-  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
   Tensor scratch;
   if (need > 0) scratch = stream_workspace(q.device(), stream, need, {0, FLASH_PACKED_TICKET_BYTES});
   raise(flash_fwd_packed(&a, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
@@ -272,13 +281,13 @@ std::tuple<Tensor, Tensor> decode_paged(const Tensor& q, const Tensor& k_cache, 
   }
   check_device(q, {&k_cache, &v_cache, &page_table, &seq_lens, &or_none(k_scale), &or_none(v_scale), &or_none(out_given), &or_none(workspace)});
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const auto stream = stream_of(q.device(), sync);
   Tensor o = output_for(q, out_given), lse, scratch;
   a.o = o.data_ptr();
   if (return_lse) {
     lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
     a.lse = static_cast<float*>(lse.data_ptr());
   }
-  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index());
   if (need > 0) scratch = workspace ? *workspace : stream_workspace(q.device(), stream, need, {FLASH_DECODE_PARTS_BYTES, -1});
   raise(flash_decode_paged(&a, &c, need > 0 ? scratch.data_ptr() : nullptr, need, stream.stream()));
   modified({&or_none(out_given), &or_none(workspace)});
@@ -311,7 +320,7 @@ void cache_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const
   a.v_head_stride = v.stride(1);
   check_device(k, {&v, &k_cache, &v_cache, &page_table, &seq_lens, &or_none(cu_seqlens), &or_none(k_scale), &or_none(v_scale)});
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(k.device());
-  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(k.device().index());
+  const auto stream = stream_of(k.device(), sync);
   raise(flash_cache_append(&a, &c, stream.stream()));
   modified({&k_cache, &v_cache});
   if (sync) wait_for(stream);

@@ -335,3 +335,30 @@ def test_scales_of_values_of_any_size(fa, dtype, scale, lens):
     vs = torch.tensor([scale])
     got = fa.decode_paged(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softmax_scale=0.005, v_scale=vs.cuda())
     bounds.check_decoding(got, q, rows, lens, 0.005, None, vs)
+
+
+def test_waiting_inside_a_capture_is_refused(fa):
+    """Each operator with its default sync=True: an error in front of the launch, and the capture goes on."""
+    lens = [300, 2000]
+    kc, vc, table, _ = filled(lens, 16, 2, 64, F16, seed=3)
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(n, h, 64, generator=gen).half().cuda() for n, h in ((2, 4), (2, 2), (2, 2)))
+    rest = (kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    want = fa.decode_paged(q, *rest), fa.forward_packed(q, k, v, cu)
+    out = torch.empty_like(q), torch.empty_like(q)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        fa.decode_paged(q, *rest, out=out[0], sync=False)
+        for call in (lambda: fa.decode_paged(q, *rest, out=out[0]), lambda: fa.forward_packed(q, k, v, cu, out=out[1]),
+                     lambda: fa.cache_append(k, v, *rest)):
+            with pytest.raises(ValueError, match="sync=False"):
+                call()
+        fa.forward_packed(q, k, v, cu, out=out[1], sync=False)
+    for _ in range(3):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
